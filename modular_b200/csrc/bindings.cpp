@@ -1376,4 +1376,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("profile", &PyDecoderExecutor::profile);
   mb::bind_runtime(m);
   mb::bind_layers(m);
+  mb::bind_kv8(m);
 }

@@ -16,5 +16,6 @@ int num_sms();
 }  // namespace bind
 
 void bind_layers(pybind11::module_& m);           // bindings_layers.cpp
+void bind_kv8(pybind11::module_& m);              // bindings_kv8.cpp
 
 }  // namespace mb

@@ -1,0 +1,180 @@
+// Bindings of the 8-bit paged key/value cache.
+#include "bindings.h"
+
+#include <c10/cuda/CUDAGuard.h>
+
+#include "common/api.h"
+
+namespace py = pybind11;
+using torch::Tensor;
+using namespace mb::bind;
+typedef c10::optional<Tensor> Opt;
+
+namespace {
+
+int dtype_code(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kFloat: return 1;
+    case at::kHalf: return 2;
+    default: break;
+  }
+  TORCH_CHECK(false, what, ": bf16, fp16 or fp32 expected, got ", t.scalar_type());
+}
+
+void on_device(const Tensor& t, const Tensor& like, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), what, " must be on ", like.device());
+}
+
+// The error word lies on the device that was current when it was made; kernels on another device go without.
+int* error_flag_on(int device) {
+  int* f = error_flag();
+  static const int where = [f] {
+    cudaPointerAttributes at = {};
+    return cudaPointerGetAttributes(&at, f) == cudaSuccess ? at.device : -1;
+  }();
+  return where == device ? f : nullptr;
+}
+
+int ld_of(const Tensor& t, int64_t cols, const char* what) {
+  TORCH_CHECK(t.dim() == 2 && t.size(1) >= cols && (t.stride(1) == 1 || t.size(1) == 1), what, ": a matrix of at least ", cols,
+              " columns with unit column stride");
+  TORCH_CHECK(t.stride(0) >= cols || t.size(0) <= 1, what, ": rows overlap");
+  TORCH_CHECK(t.stride(0) < (1ll << 31), what, ": row stride");
+  const int64_t ld = t.size(0) <= 1 ? (t.size(1) + 7) / 8 * 8 : t.stride(0);      // (one row has no stride to speak of)
+  TORCH_CHECK(ld % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, what, ": rows must start on 16 bytes");
+  return static_cast<int>(ld);
+}
+
+const int32_t* i32(const Tensor& t, int64_t n, const Tensor& like, const char* what) {
+  on_device(t, like, what);
+  TORCH_CHECK(t.is_contiguous() && t.scalar_type() == at::kInt && t.numel() >= n, what, ": int32, at least ", n, " values, contiguous");
+  return t.data_ptr<int32_t>();
+}
+
+MbFp8Cache cache_of(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int n_kv, int hd, const Tensor& like) {
+  MbFp8Cache c = {};
+  auto plane = [&](const Tensor& t, const Tensor& s, const char* what) {
+    on_device(t, like, what);
+    on_device(s, like, what);
+    TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn && t.dim() == 4, what, "_cache: float8_e4m3fn [pages, kv heads, page, head_dim]");
+    TORCH_CHECK(t.size(1) == n_kv && t.size(3) == hd, what, "_cache: ", n_kv, " heads of ", hd, " expected, got ", t.sizes());
+    TORCH_CHECK(t.stride(3) == 1 && t.stride(2) == hd, what, "_cache: the rows of a head lie together");
+    TORCH_CHECK(s.scalar_type() == at::kByte && s.dim() == 3 && s.size(0) == t.size(0) && s.size(1) == t.size(1) && s.size(2) == t.size(2) &&
+                    s.stride(2) == 1, what, "_scale: uint8 [pages, kv heads, page] with unit stride along the page");
+    TORCH_CHECK(t.size(2) >= 16 && t.size(2) % 16 == 0, "page size ", t.size(2), " is no multiple of 16");
+    TORCH_CHECK(t.size(0) >= 1 && t.size(0) < (1ll << 31), what, "_cache: pages");
+  };
+  plane(k, ks, "k");
+  plane(v, vs, "v");
+  TORCH_CHECK(v.size(0) == k.size(0) && v.size(2) == k.size(2), "k_cache and v_cache differ in pages");
+  c.k = k.data_ptr(); c.v = v.data_ptr();
+  c.ks = ks.data_ptr<uint8_t>(); c.vs = vs.data_ptr<uint8_t>();
+  c.k_page = k.stride(0); c.k_head = k.stride(1); c.v_page = v.stride(0); c.v_head = v.stride(1);
+  c.ks_page = ks.stride(0); c.ks_head = ks.stride(1); c.vs_page = vs.stride(0); c.vs_head = vs.stride(1);
+  // a stride that is never taken need not be aligned
+  if (c.pages = static_cast<int>(k.size(0)); c.pages == 1) c.k_page = c.v_page = c.ks_page = c.vs_page = 0;
+  if (n_kv == 1) c.k_head = c.v_head = c.ks_head = c.vs_head = 0;
+  c.page_size = static_cast<int>(k.size(2));
+  return c;
+}
+
+void rope_kv_store_fp8(const Tensor& qkv, const Tensor& positions, const Tensor& slots, const Opt& cos_sin, Tensor& k_cache, Tensor& v_cache,
+                       Tensor& k_scale, Tensor& v_scale, int n_q, int n_kv, int hd, bool interleaved, int rot, Tensor& q_out) {
+  need_cuda(qkv, "qkv");
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  const int dt = dtype_code(qkv, "qkv");
+  const int64_t T = qkv.size(0);
+  const MbFp8Cache c = cache_of(k_cache, v_cache, k_scale, v_scale, n_kv, hd, qkv);
+  const int ld = ld_of(qkv, static_cast<int64_t>(n_q + 2 * n_kv) * hd, "qkv");
+  on_device(q_out, qkv, "q_out");
+  TORCH_CHECK(q_out.scalar_type() == qkv.scalar_type() && q_out.size(0) >= T, "q_out: a row per token, of the type of qkv");
+  const int ldq = ld_of(q_out, static_cast<int64_t>(n_q) * hd, "q_out");
+  on_device(slots, qkv, "slots");
+  TORCH_CHECK(slots.is_contiguous() && slots.scalar_type() == at::kLong && slots.numel() >= T, "slots: int64, one per token");
+  const float* cs = nullptr;
+  int n_pos = 0;
+  if (rot > 0) {
+    TORCH_CHECK(cos_sin.has_value() && cos_sin->defined(), "cos_sin is needed to rotate");
+    on_device(*cos_sin, qkv, "cos_sin");
+    TORCH_CHECK(cos_sin->is_contiguous() && cos_sin->scalar_type() == at::kFloat && cos_sin->dim() == 2 && cos_sin->size(1) == rot,
+                "cos_sin: fp32 [positions, ", rot, "]");
+    cs = cos_sin->data_ptr<float>();
+    n_pos = static_cast<int>(cos_sin->size(0));
+  }
+  TORCH_CHECK(T < (1ll << 31), "tokens");
+  check_rc(mb_rope_kv_store_fp8(qkv.data_ptr(), ld, q_out.data_ptr(), ldq, dt, i32(positions, T, qkv, "positions"), slots.data_ptr<int64_t>(), cs,
+                                n_pos, &c, static_cast<int>(T), n_q, n_kv, hd, rot, interleaved, error_flag_on(qkv.get_device()), cur_stream()),
+           "rope_kv_store_fp8");
+}
+
+void kv_load_fp8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, const Tensor& block_table,
+                 const Tensor& kv_start, const Tensor& kv_len, int64_t rows, Tensor& k_out, Tensor& v_out) {
+  need_cuda(k_cache, "k_cache");
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  TORCH_CHECK(k_cache.dim() == 4, "k_cache: 4-D");
+  const int n_kv = k_cache.size(1), hd = k_cache.size(3);
+  const MbFp8Cache c = cache_of(k_cache, v_cache, k_scale, v_scale, n_kv, hd, k_cache);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.is_contiguous(), "block_table: int32 [sequences, pages], contiguous");
+  const int64_t B = block_table.size(0);
+  for (Tensor* t : {&k_out, &v_out}) {
+    on_device(*t, k_cache, "output");
+    TORCH_CHECK(t->is_contiguous() && t->dim() == 3 && t->size(0) >= rows && t->size(1) == n_kv && t->size(2) == hd &&
+                    t->scalar_type() == k_out.scalar_type() && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0,
+                "outputs: contiguous [rows, kv heads, head_dim] of one type");
+  }
+  check_rc(mb_kv_load_fp8(&c, i32(block_table, 0, k_cache, "block_table"), static_cast<int>(block_table.size(1)), i32(kv_start, B, k_cache, "kv_start"),
+                          i32(kv_len, B, k_cache, "kv_len"), static_cast<int>(B), rows, n_kv, hd, k_out.data_ptr(), v_out.data_ptr(),
+                          dtype_code(k_out, "output"), error_flag_on(k_cache.get_device()), cur_stream()),
+           "kv_load_fp8");
+}
+
+void paged_attention_fp8(const Tensor& q, Tensor& out, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                         const Tensor& block_table, const Tensor& q_start, const Tensor& q_len, const Tensor& kv_len, const Opt& tile_seq,
+                         const Opt& tile_q0, const Opt& decode_seq, int n_q, int n_kv, int hd, double scale) {
+  need_cuda(q, "q");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const MbFp8Cache c = cache_of(k_cache, v_cache, k_scale, v_scale, n_kv, hd, q);
+  MbFp8Attention a = {};
+  a.dtype = dtype_code(q, "q");
+  a.ldq = ld_of(q, static_cast<int64_t>(n_q) * hd, "q");
+  on_device(out, q, "out");
+  TORCH_CHECK(out.scalar_type() == q.scalar_type() && out.size(0) >= q.size(0), "out: a row per row of q, of its type");
+  a.ldo = ld_of(out, static_cast<int64_t>(n_q) * hd, "out");
+  a.q = q.data_ptr(); a.out = out.data_ptr();
+  TORCH_CHECK(block_table.dim() == 2 && block_table.is_contiguous(), "block_table: int32 [sequences, pages], contiguous");
+  const int64_t B = block_table.size(0);
+  a.block_table = i32(block_table, 0, q, "block_table");
+  a.bt_stride = static_cast<int>(block_table.size(1));
+  a.q_start = i32(q_start, B, q, "q_start"); a.q_len = i32(q_len, B, q, "q_len"); a.kv_len = i32(kv_len, B, q, "kv_len");
+  auto part = [&](const Opt& t, const char* what, int* n) -> const int32_t* {
+    if (!t.has_value() || !t->defined() || t->numel() == 0) return nullptr;
+    if (n) *n = static_cast<int>(t->numel());
+    return i32(*t, 1, q, what);
+  };
+  a.tile_seq = part(tile_seq, "tile_seq", &a.n_tiles);
+  int n0 = 0;
+  a.tile_q0 = part(tile_q0, "tile_q0", &n0);
+  TORCH_CHECK(n0 == a.n_tiles, "tile_seq and tile_q0 differ in length");
+  a.decode_seq = part(decode_seq, "decode_seq", &a.n_decode);
+  a.T = static_cast<int>(q.size(0)); a.B = static_cast<int>(B);
+  a.n_q = n_q; a.n_kv = n_kv; a.head_dim = hd; a.scale = static_cast<float>(scale);
+  a.err = error_flag_on(q.get_device());
+  // The partial results of rows whose keys are shared out: taken from the allocator for each call, so that calls on several
+  // streams and captured graphs never share them.
+  a.ws_bytes = mb_paged_attention_fp8_workspace(a.T, a.B, a.n_tiles, a.n_decode, n_q, n_kv, hd, num_sms());
+  Tensor ws;
+  if (a.ws_bytes > 0) {
+    ws = torch::empty({static_cast<int64_t>(a.ws_bytes)}, q.options().dtype(at::kByte));
+    a.ws = ws.data_ptr();
+  }
+  check_rc(mb_paged_attention_fp8(&a, &c, num_sms(), cur_stream()), "paged_attention_fp8");
+}
+
+}  // namespace
+
+void mb::bind_kv8(py::module_& m) {
+  m.def("rope_kv_store_fp8", &rope_kv_store_fp8);
+  m.def("kv_load_fp8", &kv_load_fp8);
+  m.def("paged_attention_fp8", &paged_attention_fp8);
+}

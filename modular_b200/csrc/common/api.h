@@ -574,6 +574,36 @@ int mb_apply_penalties(float* logits, int rows, int vocab, int ld, const int32_t
                        const int32_t* cnt, const int32_t* offsets, const float* freq_pen,
                        const float* pres_pen, const float* rep_pen, cudaStream_t stream);
 
+// ---- 8-bit paged key/value cache (kv_fp8.cu, attention_fp8.cu) --------------------------------------------------
+// A row (a token's key or value of one head) is head_dim e4m3 codes and one exponent byte: value = code * 2^(byte - 127).
+// Codes of page g, head h, offset o start at k + g * k_page + h * k_head + o * head_dim, its byte is ks[g * ks_page + h * ks_head + o];
+// all distances in bytes. 16-byte alignment of the pointers and of every distance, page_size a multiple of 16.
+typedef struct MbFp8Cache {
+  void *k, *v;
+  uint8_t *ks, *vs;
+  long long k_page, k_head, v_page, v_head, ks_page, ks_head, vs_page, vs_head;
+  int pages, page_size;
+} MbFp8Cache;
+// dtype: 0 bf16, 1 fp32, 2 fp16
+int mb_rope_kv_store_fp8(const void* qkv, int ld, void* q_out, int ldq, int dtype, const int32_t* positions, const int64_t* slots,
+                         const float* cos_sin, int n_positions, const MbFp8Cache* cache, int T, int n_q, int n_kv, int head_dim,
+                         int rot_dims, int interleaved, int* err, cudaStream_t stream);
+int mb_kv_load_fp8(const MbFp8Cache* cache, const int32_t* block_table, int bt_stride, const int32_t* kv_start, const int32_t* kv_len,
+                   int B, long long rows, int n_kv, int head_dim, void* k_out, void* v_out, int dtype, int* err, cudaStream_t stream);
+typedef struct MbFp8Attention {
+  const void* q;               // [T, ldq], n_q * head_dim columns first
+  void* out;                   // [T, ldo]
+  const int32_t *block_table, *q_start, *q_len, *kv_len;
+  const int32_t *tile_seq, *tile_q0, *decode_seq;   // plan: tiles of up to 64 rows, and sequences of up to 16 rows
+  void* ws;                    // mb_paged_attention_fp8_workspace bytes
+  size_t ws_bytes;
+  int* err;
+  int ldq, ldo, dtype, bt_stride, T, B, n_tiles, n_decode, n_q, n_kv, head_dim;
+  float scale;
+} MbFp8Attention;
+size_t mb_paged_attention_fp8_workspace(int T, int B, int n_tiles, int n_decode, int n_q, int n_kv, int head_dim, int num_sms);
+int mb_paged_attention_fp8(const MbFp8Attention* a, const MbFp8Cache* cache, int num_sms, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,156 @@
+// Causal attention over the 8-bit paged cache (layout and meaning of a row: kv_fp8.cu).
+//
+//   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale * q_i . k_j),  j <= kv_len - q_len + i
+//
+// Queries are the last q_len tokens of their sequence; a row without keys is zero.
+//
+//   attn_rows_kernel    any head width up to 256 and any group of heads, fp32 queries too: on the CUDA cores
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../common/api.h"
+#include "../common/launch.h"
+#include "../common/ptx.cuh"
+
+namespace mb {
+namespace a8 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float pow2_byte(uint8_t b) { return __uint_as_float(b == 0 ? 0x400000u : static_cast<uint32_t>(b) << 23); }
+__device__ __forceinline__ float2 two_codes(uint32_t w) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3)));
+}
+
+struct RowsParams {
+  MbFp8Attention a;
+  MbFp8Cache c;
+};
+
+// One block per (token, query head); each of four warps takes 32 keys at a time: a lane per key for the scores, a lane per
+// HD / 32 columns for the values; running maximum and sum per warp, joined at the end. Bound by its loads of K, which are not shared between
+// rows: it serves the sizes the tensor-core kernels do not take.
+template <typename T>
+__global__ void __launch_bounds__(128) attn_rows_kernel(const RowsParams p) {
+  __shared__ float sq[256];
+  __shared__ float so[4][256];
+  __shared__ float sml[4][2];
+  __shared__ int s_seq;
+  pdl_wait();
+  const MbFp8Attention& a = p.a;
+  const int row = blockIdx.x, head = blockIdx.y, kvh = head / (a.n_q / a.n_kv), hd = a.head_dim;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) s_seq = -1;
+  __syncthreads();
+  for (int s = tid; s < a.B; s += 128)
+    if (row >= a.q_start[s] && row - a.q_start[s] < a.q_len[s]) s_seq = s;
+  for (int i = tid; i < hd; i += 128)
+    sq[i] = static_cast<float>(static_cast<const T*>(a.q)[static_cast<int64_t>(row) * a.ldq + static_cast<int64_t>(head) * hd + i]) * (a.scale * kLog2e);
+  __syncthreads();
+  const int seq = s_seq;
+  if (seq < 0) return;                               // a row of no sequence stays as it is
+  const int keys = a.kv_len[seq] - a.q_len[seq] + (row - a.q_start[seq]) + 1;
+  const int per = hd / 32, rest = hd % 32;           // columns of a lane: lane + 32 i
+  float o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const int32_t* bt = a.block_table + static_cast<int64_t>(seq) * a.bt_stride;
+  for (int k0 = warp * 32; k0 < keys; k0 += 128) {
+    const int j = k0 + lane;
+    float s = -INFINITY;
+    int page = -1, off = 0;
+    if (j < keys) {
+      page = j / p.c.page_size < a.bt_stride ? bt[j / p.c.page_size] : -1;
+      off = j % p.c.page_size;
+      if (page < 0 || page >= p.c.pages) {
+        if (a.err) atomicCAS(a.err, 0, 731);
+        page = -1;
+      } else {
+        const uint8_t* kr = static_cast<const uint8_t*>(p.c.k) + page * p.c.k_page + kvh * p.c.k_head + static_cast<int64_t>(off) * hd;
+        float acc = 0.f;
+        for (int c = 0; c < hd; c += 16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(kr + c);
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 f = two_codes(words[i >> 1] >> (16 * (i & 1)));
+            acc = fmaf(f.x, sq[c + 2 * i], acc);
+            acc = fmaf(f.y, sq[c + 2 * i + 1], acc);
+          }
+        }
+        s = acc * pow2_byte(p.c.ks[page * p.c.ks_page + kvh * p.c.ks_head + off]);
+      }
+    }
+    float mx = s;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float mn = fmaxf(m, mx);
+    const float keep = m == -INFINITY ? 0.f : exp2f(m - mn);
+    const float w = page < 0 ? 0.f : exp2f(s - mn);
+    m = mn;
+    l = l * keep + w;                                // of this lane's keys
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= keep;
+    const float wv = page < 0 ? 0.f : w * pow2_byte(p.c.vs[page * p.c.vs_page + kvh * p.c.vs_head + off]);
+    for (int n = 0; n < 32; ++n) {
+      const int pg = __shfl_sync(0xffffffffu, page, n), of = __shfl_sync(0xffffffffu, off, n);
+      const float pw = __shfl_sync(0xffffffffu, wv, n);
+      if (pg < 0) continue;
+      const uint8_t* vr = static_cast<const uint8_t*>(p.c.v) + pg * p.c.v_page + kvh * p.c.v_head + static_cast<int64_t>(of) * hd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < per || (i == per && lane < rest)) o[i] = fmaf(pw, two_codes(vr[lane + 32 * i]).x, o[i]);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < per || (i == per && lane < rest)) so[warp][lane + 32 * i] = o[i];
+  if (lane == 0) { sml[warp][0] = m; sml[warp][1] = l; }
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, sml[w][0]);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = sml[w][0] == -INFINITY ? 0.f : exp2f(sml[w][0] - top);
+    sum += f[w] * sml[w][1];
+  }
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);     // (NaN stays)
+  for (int i = tid; i < hd; i += 128) {
+    float acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) acc += f[w] == 0.f ? 0.f : f[w] * so[w][i];
+    static_cast<T*>(a.out)[static_cast<int64_t>(row) * a.ldo + static_cast<int64_t>(head) * hd + i] = static_cast<T>(acc * inv);
+  }
+}
+
+}  // namespace a8
+}  // namespace mb
+
+using namespace mb;
+
+extern "C" size_t mb_paged_attention_fp8_workspace(int T, int B, int n_tiles, int n_decode, int n_q, int n_kv, int head_dim, int num_sms) {
+  (void)T; (void)B; (void)n_tiles; (void)n_decode; (void)n_q; (void)n_kv; (void)head_dim; (void)num_sms;
+  return 0;
+}
+
+extern "C" int mb_paged_attention_fp8(const MbFp8Attention* a, const MbFp8Cache* c, int num_sms, cudaStream_t stream) {
+  using namespace mb::a8;
+  (void)num_sms;
+  if (a->T <= 0 || a->B <= 0) return MB_OK;
+  if (a->n_kv < 1 || a->n_q < 1 || a->n_q % a->n_kv || a->head_dim < 16 || a->head_dim > 256 || a->head_dim % 16) return MB_ERR_SHAPE;
+  if (c->page_size < 16 || c->page_size % 16 || c->pages < 1 || !(a->scale > 0.f) || a->n_q > 65535) return MB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->ks) | reinterpret_cast<uintptr_t>(c->vs) |
+       static_cast<uintptr_t>(c->k_page | c->k_head | c->v_page | c->v_head | c->ks_page | c->ks_head | c->vs_page | c->vs_head)) & 15)
+    return MB_ERR_ALIGN;
+  if (((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15) || a->ldq % 8 || a->ldo % 8) return MB_ERR_ALIGN;
+  RowsParams p = {*a, *c};
+  auto kern = a->dtype == 0 ? attn_rows_kernel<__nv_bfloat16> : a->dtype == 1 ? attn_rows_kernel<float> : attn_rows_kernel<__half>;
+  return launch_k(kern, dim3(a->T, a->n_q), dim3(128), 0, stream, p) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+}

@@ -23,6 +23,7 @@ __all__ = [
     "linear", "linear_swiglu", "rms_norm", "add_rms_norm", "silu_mul", "embedding",
     "rope_kv_store", "paged_attention", "build_attention_plan", "argmax", "sample",
     "apply_penalties", "gelu_tanh", "xielu", "tanh", "softcap", "sigmoid_gate", "gemm_workspace", "check_device_error", "linear_decode", "decode_gemm_workspace",
+    "fp8_cache_views", "rope_kv_store_fp8", "kv_load_fp8", "paged_attention_fp8",
 ]
 
 _WORKSPACES: dict[int, torch.Tensor] = {}
@@ -388,6 +389,98 @@ def paged_attention(q, k_cache, v_cache, block_table, q_start, q_len, kv_len, n_
     else:
         _lib().paged_attention(q, out, k_cache, v_cache, block_table, q_start, q_len, kv_len,
                                plan[0], plan[1], plan[2], n_q, n_kv, head_dim, scale)
+    return out
+
+
+# ------------------------------------------------------------------ 8-bit key/value cache
+# A row (a token's key or value of one head) is head_dim e4m3 codes and one exponent byte, value = code * 2^(byte - 127). The exponent is the
+# smallest (but not under -100) with which the row's largest finite magnitude is at most 448; codes are rounded to the nearest, ties to
+# even; what is not finite is held as NaN. ``k_cache`` / ``v_cache``: float8_e4m3fn [pages, kv heads, page, head_dim], rows of a head together;
+# ``k_scale`` / ``v_scale``: uint8 [pages, kv heads, page]. Pages and heads may lie at any distance that is a multiple of 16 bytes.
+def fp8_cache_views(kv, layer: int):
+    """``(k_cache, v_cache, k_scale, v_scale)`` of one layer of a cache tensor uint8 [pages, 2, layers, kv heads, page, head_dim + 1] (what
+    ``KVCacheParams(kv_format="float8_e4m3fn")`` allocates): a head of a page is its page x head_dim codes, then its page exponents."""
+    if kv.dim() != 6 or kv.dtype != torch.uint8 or not kv.is_contiguous() or kv.shape[1] != 2:
+        raise ValueError("an 8-bit cache is a contiguous uint8 tensor [pages, 2, layers, kv heads, page, head_dim + 1]")
+    pages, _, layers, heads, page, hd1 = kv.shape
+    if not 0 <= layer < layers:
+        raise ValueError(f"layer {layer} of {layers}")
+    flat, hd = kv.view(torch.float8_e4m3fn), hd1 - 1
+    at = [plane * kv.stride(1) + layer * kv.stride(2) for plane in (0, 1)]
+    codes = [flat.as_strided((pages, heads, page, hd), (kv.stride(0), kv.stride(3), hd, 1), a) for a in at]
+    scales = [kv.as_strided((pages, heads, page), (kv.stride(0), kv.stride(3), 1), a + page * hd) for a in at]
+    return codes[0], codes[1], scales[0], scales[1]
+
+
+def _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, n_kv, head_dim):
+    for name, c, s in (("k", k_cache, k_scale), ("v", v_cache, v_scale)):
+        if c.dtype != torch.float8_e4m3fn or c.dim() != 4 or s.dtype != torch.uint8 or tuple(s.shape) != tuple(c.shape[:3]):
+            raise ValueError(f"{name}_cache: float8_e4m3fn [pages, kv heads, page, head_dim] with uint8 exponents [pages, kv heads, page]")
+        if c.shape[1] != n_kv or c.shape[3] != head_dim or c.shape[2] % 16:
+            raise ValueError(f"{name}_cache: {n_kv} heads of {head_dim} in pages of a multiple of 16 expected, got {tuple(c.shape)}")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache differ")
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise ValueError(f"head_dim {head_dim}: a multiple of 16 up to 256")
+
+
+def rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale, v_scale, n_q, n_kv, head_dim, interleaved=False, rot_dims=None,
+                      q_out=None):
+    """Rotates queries and keys of ``qkv`` [T, (n_q + 2 n_kv) * head_dim or more] and writes keys and values to the 8-bit cache.
+
+    ``cos_sin`` fp32 [positions, rot_dims] (cosines, then sines; from :func:`nn.rotary_embedding.cos_sin_table`, whatever its scaling);
+    ``rot_dims`` (default head_dim, 0: no rotation) columns of a head turn, in pairs ``rot_dims / 2`` apart or neighbouring
+    (``interleaved``). ``slots`` int64 [T]: page * page_size + offset, negative: the token is not stored. Two tokens of a call must not
+    name one slot. The rotated queries replace those in ``qkv``, or go to ``q_out`` (then ``qkv`` stays as it is); they are returned
+    as [T, n_q * head_dim]. Rows are rounded once, from the rotation's exact result. A position or slot out of range is reported by
+    :func:`check_device_error` and its row is not rotated or not stored."""
+    rot = head_dim if rot_dims is None else int(rot_dims)
+    if rot % 2 or not 0 <= rot <= head_dim:
+        raise ValueError(f"rot_dims {rot} of {head_dim}")
+    q = qkv if q_out is None else q_out
+    if qkv.is_cuda:
+        _lib().rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale, v_scale, n_q, n_kv, head_dim, interleaved, rot, q)
+    else:
+        _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, n_kv, head_dim)
+        ref.rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale, v_scale, n_q, n_kv, head_dim, interleaved, rot, q)
+    return q[: qkv.shape[0], : n_q * head_dim]
+
+
+def kv_load_fp8(k_cache, v_cache, k_scale, v_scale, block_table, kv_start, kv_len, rows, dtype=torch.bfloat16, out=None):
+    """Keys and values of whole sequences read back from the 8-bit cache: ``(k, v)``, each [rows, kv heads, head_dim] of ``dtype`` (bf16, fp16 or
+    fp32; bf16 and fp32 hold them exactly). Tokens [0, kv_len[s]) of sequence s go to the rows from ``kv_start[s]`` on (rising);
+    rows that belong to no sequence are zeros. ``out``: a pair of tensors to fill instead, whose rows from ``rows`` on stay as they are."""
+    n_kv, hd = k_cache.shape[1], k_cache.shape[3]
+    if out is None:
+        out = tuple(torch.empty(rows, n_kv, hd, dtype=dtype, device=k_cache.device) for _ in range(2))
+    if k_cache.is_cuda:
+        _lib().kv_load_fp8(k_cache, v_cache, k_scale, v_scale, block_table, kv_start, kv_len, rows, out[0], out[1])
+    else:
+        _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, n_kv, hd)
+        ref.kv_load_fp8(k_cache, v_cache, k_scale, v_scale, block_table, kv_start, kv_len, out[0], out[1], rows)
+    return tuple(out)
+
+
+def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, q_start, q_len, kv_len, n_q, n_kv, head_dim, scale, plan=None, out=None):
+    """Ragged causal attention over the 8-bit cache. ``q`` [T, n_q * head_dim or more], rotated; its type (bf16, fp16, fp32) is that of the
+    output. Sequence s has rows [q_start, q_start + q_len) of ``q``, its last ``q_len`` of ``kv_len`` tokens; a row without keys is zero, and
+    rows of no sequence stay as they are. ``plan``: :func:`build_attention_plan` on the device (made here, with a copy of ``q_len`` to the host,
+    if None). Accumulates in fp32. ``scale`` > 0. A page number out of range is reported by :func:`check_device_error`."""
+    if not scale > 0:
+        raise ValueError(f"scale {scale}: must be positive")
+    if n_kv < 1 or n_q % n_kv:
+        raise ValueError(f"{n_q} query heads over {n_kv}")
+    if out is None:
+        out = torch.empty(q.shape[0], n_q * head_dim, dtype=q.dtype, device=q.device)
+    if not q.is_cuda:
+        _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, n_kv, head_dim)
+        ref.paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, q_start, q_len, kv_len, n_q, n_kv, head_dim, scale, out)
+        return out
+    if plan is None:
+        parts = build_attention_plan(q_len.cpu().numpy(), n_q, n_kv)
+        plan = tuple(torch.from_numpy(a).to(q.device) if a.size else None for a in parts)
+    _lib().paged_attention_fp8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, q_start, q_len, kv_len, plan[0], plan[1], plan[2], n_q, n_kv,
+                               head_dim, float(scale))
     return out
 
 

@@ -294,6 +294,90 @@ def linear_fp8_blockscaled(xq, xs, wq, ws, residual=None, out_dtype=torch.bfloat
     return y
 
 
+# ---------------------------------------------------------------------- 8-bit paged key/value cache
+FP8_ROW_LEAST_EXP = -100
+
+
+def quant_fp8_rows(x):
+    """Rows of the 8-bit cache: (e4m3 codes of x's shape, exponent bytes uint8 of x's shape without the last dimension) with
+    ``x ~ code * 2^(byte - 127)``. The exponent is the smallest one, but not under -100, with which the largest finite magnitude of a row is
+    at most 448; codes are the nearest e4m3 numbers, ties to even; what is not finite is held as NaN. In 64 bits throughout."""
+    xf = x.double()
+    fine = torch.isfinite(xf)
+    amax = torch.where(fine, xf.abs(), torch.zeros_like(xf)).amax(-1)
+    frac, e = torch.frexp((amax / FP8_MAX).clamp_min(1e-200))         # amax / 448 = frac * 2^e, frac in [0.5, 1)
+    e = torch.where(frac == 0.5, e - 1, e).clamp_min(FP8_ROW_LEAST_EXP)
+    y = xf * _pow2_f64(-e).unsqueeze(-1)
+    step = _pow2_f64((torch.frexp(y)[1] - 4).clamp_min(-9))           # distance of e4m3 numbers around y
+    y = torch.where(fine, torch.round(y / step) * step, torch.full_like(y, math.nan))
+    return y.float().to(torch.float8_e4m3fn), (e + 127).to(torch.uint8)
+
+
+def _pow2_f64(e):
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def dequant_fp8_rows(codes, scale_bytes, dtype=torch.float32):
+    """Values of rows of the 8-bit cache (exact in fp32 and bf16)."""
+    return (codes.double() * _pow2_f64(scale_bytes.long() - 127).unsqueeze(-1)).to(dtype)
+
+
+def rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale, v_scale, n_q, n_kv, head_dim, interleaved, rot_dims, q_out):
+    T = qkv.shape[0]
+    x = qkv[:, : (n_q + 2 * n_kv) * head_dim].reshape(T, n_q + 2 * n_kv, head_dim).double()
+    if rot_dims:
+        cs = cos_sin[positions.long()].double().unsqueeze(1)
+        c, s = cs[..., : rot_dims // 2], cs[..., rot_dims // 2:]
+        turn = x[:, : n_q + n_kv, :rot_dims]
+        if interleaved:
+            a, b = turn[..., 0::2].clone(), turn[..., 1::2].clone()
+            turn[..., 0::2], turn[..., 1::2] = a * c - b * s, b * c + a * s
+        else:
+            a, b = turn[..., : rot_dims // 2].clone(), turn[..., rot_dims // 2:].clone()
+            turn[..., : rot_dims // 2], turn[..., rot_dims // 2:] = a * c - b * s, b * c + a * s
+    q_out[:T, : n_q * head_dim] = x[:, :n_q].reshape(T, -1).to(qkv.dtype)
+    page = k_cache.shape[2]
+    ok = slots[:T] >= 0
+    pg, off = slots[:T][ok] // page, slots[:T][ok] % page
+    for part, cache, scale in ((x[:, n_q: n_q + n_kv], k_cache, k_scale), (x[:, n_q + n_kv:], v_cache, v_scale)):
+        codes, e = quant_fp8_rows(part[ok])
+        cache.view(torch.uint8)[pg, :, off] = codes.view(torch.uint8)
+        scale[pg, :, off] = e
+
+
+def _fp8_rows_of(cache, scale, pages, n, dtype):
+    """Rows [0, n) of a sequence: [n, heads, head_dim]."""
+    pages = pages[: -(-n // cache.shape[2])].long()
+    v = dequant_fp8_rows(cache.view(torch.uint8)[pages].view(torch.float8_e4m3fn), scale[pages], dtype)
+    return v.transpose(1, 2).reshape(-1, cache.shape[1], cache.shape[3])[:n]
+
+
+def kv_load_fp8(k_cache, v_cache, k_scale, v_scale, block_table, kv_start, kv_len, k_out, v_out, rows):
+    for out, cache, scale in ((k_out, k_cache, k_scale), (v_out, v_cache, v_scale)):
+        out[:rows] = 0
+        for s in range(block_table.shape[0]):
+            a, n = int(kv_start[s]), int(kv_len[s])
+            if n > 0:
+                out[a: a + n] = _fp8_rows_of(cache, scale, block_table[s], n, out.dtype)
+
+
+def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, q_start, q_len, kv_len, n_q, n_kv, head_dim, scale, out):
+    for s in range(block_table.shape[0]):
+        qs, ql, kl = int(q_start[s]), int(q_len[s]), int(kv_len[s])
+        if ql <= 0:
+            continue
+        o = torch.zeros(ql, n_q, head_dim, dtype=torch.float32, device=q.device)
+        if kl > 0:
+            k, v = (_fp8_rows_of(c, e, block_table[s], kl, torch.float32).repeat_interleave(n_q // n_kv, 1)
+                    for c, e in ((k_cache, k_scale), (v_cache, v_scale)))
+            qq = q[qs: qs + ql, : n_q * head_dim].float().view(ql, n_q, head_dim)
+            hidden = torch.arange(kl, device=q.device).unsqueeze(0) > torch.arange(kl - ql, kl, device=q.device).unsqueeze(1)
+            w = torch.einsum("qhd,khd->hqk", qq, k).mul(scale).masked_fill(hidden, float("-inf"))
+            w = torch.exp(w - w.amax(-1, keepdim=True).clamp_min(-1e30))
+            o = torch.einsum("hqk,khd->qhd", w, v) / w.sum(-1).t().unsqueeze(-1).clamp_min(1e-37)      # (rows without keys: zero)
+        out[qs: qs + ql, : n_q * head_dim] = o.reshape(ql, -1).to(out.dtype)
+
+
 # ---------------------------------------------------------------------- multi-head latent attention
 def mla_kv_store(c_kv, k_rope, slots, cache):
     """Scatter one latent row per token: cache[page, offset] = [c_kv (kv_lora_rank) | k_rope].

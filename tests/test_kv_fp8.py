@@ -1,0 +1,448 @@
+"""The 8-bit paged key/value cache: rotation and store, rows read back, attention of single tokens and of chunks.
+
+The oracle is float64 throughout and shares no code with the package. Store and load are compared for equality: the codes are the
+rounded exact values. Attention is compared elementwise with
+
+    |out - o| <= eps(out) / 2 |o| + (2^-10 + 4 ds) A + n 2^-31 max|v|,     A = sum_j p_j |v_j|
+
+eps / 2 is the rounding of the output. Of the 2^-10, 2^-11 is the rounding of the probabilities to 11 bits (the sum of all is taken before it),
+2^-19 two approximate exponentials (2^-22 each) and the joining of partial sums, the rest the sums of the products with the values in fp32
+(relative errors of n 2^-24 in sum, n <= 2^12 keys here). ds is the error of a score in fp32: its d products are exact in the
+accumulator's inputs, their sum errs by d 2^-24 sum |q k| at most, and it enters numerator and denominator. The last term is
+probabilities below 2^-21 of the largest, which keep fewer than 11 bits but are off by 2^-32 of it at most.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from modular_b200 import ops
+
+gpu = pytest.mark.gpu
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def devices():
+    return [pytest.param("cpu"), pytest.param("cuda", marks=gpu)]
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error(request):
+    yield
+    if torch.cuda.is_available() and "gpu" in request.keywords:
+        torch.cuda.synchronize()
+        ops.check_device_error()
+
+
+# ------------------------------------------------------------------------------------------------------------ oracle
+GRID = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()     # the magnitudes of e4m3, rising
+
+
+def quantise(x):
+    """x float64 [..., d] on the CPU: (codes as numbers, bytes)."""
+    fine = torch.isfinite(x)
+    big = torch.where(fine, x.abs(), torch.zeros_like(x)).amax(-1)
+    e = torch.full(big.shape, -100, dtype=torch.long)
+    for k in range(-100, 122):
+        e[big > 448.0 * 2.0 ** k] = k + 1
+    y = torch.where(fine, x, torch.zeros_like(x)) / torch.tensor([2.0 ** i for i in range(-100, 130)], dtype=torch.float64)[e + 100].unsqueeze(-1)
+    a = y.abs()
+    hi = torch.searchsorted(GRID, a).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    up = (GRID[hi] - a < a - GRID[lo]) | ((GRID[hi] - a == a - GRID[lo]) & (hi % 2 == 0)) | (GRID[hi] == a)
+    q = torch.where(up, GRID[hi], GRID[lo]) * torch.where(y < 0, -1.0, 1.0)
+    return torch.where(fine, q, torch.full_like(q, math.nan)), (e + 127).to(torch.uint8)
+
+
+def rotate(x, cs, rot, interleaved):
+    """x float64 [T, heads, d], cs float64 [T, rot]."""
+    x = x.clone()
+    half = rot // 2
+    for i in range(half):
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+        c, s = cs[:, i: i + 1], cs[:, half + i: half + i + 1]
+        u, w = x[:, :, a].clone(), x[:, :, b].clone()
+        x[:, :, a], x[:, :, b] = u * c - w * s, w * c + u * s
+    return x
+
+
+class Cache:
+    """Pages of an 8-bit cache with other layers around it, so that no distance is the packed one."""
+
+    def __init__(self, pages, n_kv, page, d, device, layers=3, layer=1):
+        self.kv = torch.zeros(pages, 2, layers, n_kv, page, d + 1, dtype=torch.uint8, device=device)
+        self.views = ops.fp8_cache_views(self.kv, layer)
+        self.page = page
+
+    def fill(self, k, v):
+        """k, v float64 [pages, n_kv, page, d] on the CPU. Returns their values as held."""
+        held = []
+        for i, x in enumerate((k, v)):
+            q, b = quantise(x)
+            self.views[i].copy_(q.float().to(torch.float8_e4m3fn))
+            self.views[2 + i].copy_(b)
+            held.append(q * 2.0 ** (b.double() - 127).unsqueeze(-1))
+        return held
+
+
+def attention(q, k, v, table, q_start, q_len, kv_len, n_q, n_kv, d, scale):
+    """(out, A, largest |v|, sum |q k| scale) in float64; k, v [pages, n_kv, page, d]. Rows of no sequence are NaN in `out`."""
+    out = torch.full((q.shape[0], n_q, d), math.nan, dtype=torch.float64)
+    A, S = torch.zeros_like(out), torch.zeros(q.shape[0], n_q, 1, dtype=torch.float64)
+    big = torch.zeros_like(S)
+    for s in range(len(q_start)):
+        a, n, total = q_start[s], q_len[s], max(0, kv_len[s])
+        if n <= 0:
+            continue
+        out[a: a + n] = 0
+        pages = table[s].long()[: -(-total // k.shape[2])]
+        ks, vs = (x[pages].transpose(1, 2).reshape(-1, n_kv, d)[:total] for x in (k, v))
+        for h in range(n_q):
+            g = h // (n_q // n_kv)
+            for t in range(n):
+                seen = max(0, kv_len[s] - n + t + 1)
+                if seen == 0:
+                    continue
+                row = q[a + t, h * d: (h + 1) * d].double()
+                w = (ks[:seen, g] @ row) * scale
+                p = torch.exp(w - w.max())
+                p = p / p.sum()
+                out[a + t, h] = p @ vs[:seen, g]
+                A[a + t, h] = p @ vs[:seen, g].abs()
+                S[a + t, h] = (ks[:seen, g].abs() @ row.abs()).max() * scale
+                big[a + t, h] = vs[:seen, g].abs().max()
+    return out, A, big, S
+
+
+def check_attention(got, want, dtype, d, n_keys):
+    out, A, big, S = want
+    got = got.double().cpu()[:, : out.shape[1] * out.shape[2]].reshape(out.shape)
+    tol = torch.finfo(dtype).eps / 2 * out.abs() + (2.0 ** -10 + 4 * d * 2.0 ** -24 * S) * A + n_keys * 2.0 ** -31 * big + 1e-30
+    rows = ~out.isnan()
+    bad = ~((got - out).abs() <= tol) & rows
+    assert not bad.any(), f"{int(bad.sum())} of {int(rows.sum())}, worst {((got - out).abs() / tol)[rows].max():.2f} of the tolerance"
+
+
+def ints(a, device):
+    return torch.tensor(a, dtype=torch.int32, device=device)
+
+
+def case(new, before, n_q, n_kv, d, page, dtype, device, seed=0, stale_nan=False, ld_extra=0, tail_rows=0):
+    g = torch.Generator().manual_seed(seed)
+    total = [n + b for n, b in zip(new, before)]
+    need = [max(0, -(-t // page)) for t in total]
+    pages = sum(need) + 2
+    cache = Cache(pages, n_kv, page, d, device)
+    k = torch.randn(pages, n_kv, page, d, generator=g, dtype=torch.float64) * torch.exp2(torch.randn(n_kv, 1, d, generator=g).clamp(-2, 2).double())
+    v = torch.randn(pages, n_kv, page, d, generator=g, dtype=torch.float64) * torch.exp2(2 * torch.randn(pages, n_kv, page, 1, generator=g).double())
+    order = torch.randperm(pages, generator=g).tolist()
+    table = torch.full((len(new), max(need + [1])), order[-1], dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = torch.tensor(order[at: at + n], dtype=torch.int32)
+        at += n
+    held = cache.fill(k, v)
+    if stale_nan:       # rows past the end of every sequence, and pages of nobody: NaN codes with the largest exponent
+        used = torch.zeros(pages, page, dtype=torch.bool)
+        for i, t in enumerate(total):
+            for j in range(max(0, t)):
+                used[int(table[i, j // page]), j % page] = True
+        free = ~used.to(device)
+        for i in range(2):
+            cache.views[i].view(torch.uint8).masked_fill_(free[:, None, :, None], 0x7F)
+            cache.views[2 + i].masked_fill_(free[:, None, :], 255)
+    T = sum(max(0, n) for n in new) + tail_rows
+    start = np.cumsum([0] + [max(0, n) for n in new])[:-1].tolist()
+    q = torch.randn(T, n_q * d + ld_extra, generator=g).to(dtype).to(device)
+    return dict(cache=cache, held=held, table=table, start=start, new=new, total=total, q=q, n_q=n_q, n_kv=n_kv, d=d, scale=d ** -0.5,
+                device=device, dtype=dtype, n_keys=max(total + [1]))
+
+
+def run_attention(c, out=None, plan=None):
+    dev = c["device"]
+    return ops.paged_attention_fp8(c["q"], *c["cache"].views, c["table"].to(dev), ints(c["start"], dev), ints(c["new"], dev), ints(c["total"], dev),
+                                   c["n_q"], c["n_kv"], c["d"], c["scale"], out=out, plan=plan)
+
+
+def oracle(c):
+    return attention(c["q"].cpu(), *c["held"], c["table"], c["start"], c["new"], c["total"], c["n_q"], c["n_kv"], c["d"], c["scale"])
+
+
+# ------------------------------------------------------------------------------------------------------------ store and load
+@pytest.mark.parametrize("device", devices())
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n_q,n_kv,d,page,rot,interleaved", [
+    (4, 2, 128, 16, 128, False), (4, 2, 128, 128, 128, True), (7, 1, 64, 48, 32, False), (3, 3, 64, 64, 16, True),
+    (2, 1, 256, 32, 64, False), (1, 1, 80, 16, 20, False), (2, 2, 96, 16, 12, True), (5, 5, 16, 16, 16, False), (2, 1, 128, 16, 0, False),
+    (0, 2, 64, 16, 64, False)])
+def test_store_is_the_rounded_exact_value(n_q, n_kv, d, page, rot, interleaved, dtype, device):
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(n_q * 1000 + d + rot)
+    T, pages, n_pos = 37, 5, 300
+    x = (torch.randn(T, (n_q + 2 * n_kv) * d + 8, generator=g) * torch.exp2(3 * torch.randn(T, 1, generator=g))).to(dt)
+    pos = torch.randint(0, n_pos, (T,), generator=g).int()
+    ang = torch.rand(n_pos, max(rot, 2) // 2, generator=g) * 50
+    cs = torch.cat([ang.cos(), ang.sin()], 1)
+    cache = Cache(pages, n_kv, page, d, device)
+    cache.kv.fill_(0x5A)
+    slots = torch.randperm(pages * page, generator=g)[:T]
+    slots[3] = slots[11] = -1
+    dev = lambda t: t.to(device)  # noqa: E731
+    big = dev(x)
+    qkv = big[:, : (n_q + 2 * n_kv) * d] if d % 8 == 0 else big
+    before = big.clone()
+    q_out = torch.full((T + 2, max(n_q, 1) * d + 16), 7.0, dtype=dt, device=device)
+    got = ops.rope_kv_store_fp8(qkv, dev(pos), dev(slots), dev(cs) if rot else None, *cache.views, n_q, n_kv, d, interleaved=interleaved,
+                                rot_dims=rot, q_out=q_out)
+    assert torch.equal(big, before)                                           # with q_out nothing changes in place
+    assert (q_out[T:] == 7).all() and (q_out[:, n_q * d:] == 7).all()
+    r = x[:, : (n_q + 2 * n_kv) * d].double().view(T, -1, d)
+    if rot:
+        r = torch.cat([rotate(r[:, : n_q + n_kv], cs.double()[pos.long()], rot, interleaved), r[:, n_q + n_kv:]], 1)
+    q = r[:, :n_q].reshape(T, -1)
+    # the nearest number of the type (half a step), of a sum that errs by 2^-45 of its terms at most
+    assert ((got.cpu().double() - q).abs() <= torch.finfo(dt).eps / 2 * q.abs() + 2.0 ** -44 * x.double().abs().max()
+            + (2.0 ** -25 if dt == torch.float16 else 0)).all()
+    want_kv = torch.full_like(cache.kv, 0x5A).cpu()
+    views = ops.fp8_cache_views(want_kv, 1)
+    for i, part in enumerate((r[:, n_q: n_q + n_kv], r[:, n_q + n_kv:])):
+        codes, e = quantise(part)
+        for t in range(T):
+            if slots[t] >= 0:
+                views[i][slots[t] // page, :, slots[t] % page] = codes[t].float().to(torch.float8_e4m3fn)
+                views[2 + i][slots[t] // page, :, slots[t] % page] = e[t]
+    have = ops.fp8_cache_views(cache.kv.cpu(), 1)
+    for a, b in zip(have, views):
+        a, b = a.float(), b.float()
+        assert torch.equal(a.nan_to_num(1e9), b.nan_to_num(1e9))
+    for other in (0, 2):                                                      # the other layers
+        assert all((t.view(torch.uint8) == 0x5A).all() for t in ops.fp8_cache_views(cache.kv.cpu(), other))
+    # in place, the same numbers
+    again = ops.rope_kv_store_fp8(qkv, dev(pos), dev(slots), dev(cs) if rot else None, *cache.views, n_q, n_kv, d, interleaved=interleaved, rot_dims=rot)
+    assert torch.equal(again.float(), got.float()) and (n_q == 0 or again.data_ptr() == big.data_ptr())
+    assert torch.equal(big[:, n_q * d:], before[:, n_q * d:])
+
+
+@pytest.mark.parametrize("device", devices())
+def test_store_ties_borders_and_values_that_are_not_finite(device):
+    d, H = 64, 1
+    rows = []
+    for scale in (1.0, 2.0 ** -60, 2.0 ** 90):
+        grid = GRID.float()
+        mid = (grid[1:] + grid[:-1]) / 2                                      # every tie of e4m3, in rows whose largest value is 448
+        for i in range(0, 126, 62):
+            r = torch.zeros(d)
+            r[: len(mid[i: i + 62])] = mid[i: i + 62] * torch.where(torch.arange(len(mid[i: i + 62])) % 3 == 0, -1.0, 1.0)
+            r[63] = 448.0
+            rows.append(r * scale)
+        for top in (448.0, 449.0, 447.0, 450.0, 896.0, 448.0 * 1.0000001, 240.0, 1.75, 1.7500001):
+            rows.append(torch.cat([torch.tensor([top, -top / 3]), torch.zeros(d - 2)]) * scale)
+    rows.append(torch.zeros(d))
+    rows.append(torch.full((d,), 1e-38))
+    rows.append(torch.full((d,), -1e-30))
+    for bad in (math.inf, -math.inf, math.nan):
+        r = torch.linspace(-3, 3, d)
+        r[5] = bad
+        rows.append(r)
+    rows.append(torch.full((d,), math.nan))
+    x = torch.stack(rows)
+    T = x.shape[0]
+    cache = Cache(-(-T // 16), H, 16, d, device)
+    qkv = torch.cat([x, -x], 1).to(device)
+    ops.rope_kv_store_fp8(qkv, torch.zeros(T, dtype=torch.int32, device=device), torch.arange(T, device=device), None, *cache.views, 0, H, d, rot_dims=0)
+    for sign, codes, e in ((1, cache.views[0], cache.views[2]), (-1, cache.views[1], cache.views[3])):
+        want, byte = quantise(sign * x.double())
+        assert torch.equal(codes.cpu().float().reshape(-1, d)[:T].nan_to_num(1e9), want.float().nan_to_num(1e9))
+        assert torch.equal(e.cpu().reshape(-1)[:T], byte)
+    k, _ = ops.kv_load_fp8(*cache.views, torch.arange(cache.kv.shape[0], dtype=torch.int32, device=device).view(1, -1), ints([0], device), ints([T], device),
+                           T, torch.float32)
+    want, byte = quantise(x.double())
+    assert torch.equal(k.cpu()[:, 0].double().nan_to_num(1e300), (want * 2.0 ** (byte.double() - 127).unsqueeze(-1)).nan_to_num(1e300))
+
+
+@pytest.mark.parametrize("device", devices())
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n_kv,d,page", [(2, 128, 16), (1, 64, 48), (3, 80, 128), (1, 256, 16), (2, 16, 32)])
+def test_load_reads_rows_back(n_kv, d, page, dtype, device):
+    c = case([0] * 5, [page * 2 + 1, 0, 1, page, 5], 1, n_kv, d, page, torch.float32, device, seed=d)
+    start = [0, c["total"][0] + 2, c["total"][0] + 2, c["total"][0] + 3, c["total"][0] + 3 + page]      # a gap of two rows before the third
+    rows = start[-1] + 5 + 3                                                                                # three rows behind the last
+    out = [torch.full((rows + 4, n_kv, d), 3.0, dtype=DTYPES[dtype], device=device) for _ in range(2)]
+    got = ops.kv_load_fp8(*c["cache"].views, c["table"].to(device), ints(start, device), ints(c["total"], device), rows, out=out)
+    for x, held in zip(got, c["held"]):
+        want = torch.zeros(rows, n_kv, d, dtype=torch.float64)
+        for s, (a, n) in enumerate(zip(start, c["total"])):
+            if n:
+                want[a: a + n] = held[c["table"][s].long()[: -(-n // page)]].transpose(1, 2).reshape(-1, n_kv, d)[:n]
+        x = x.cpu()
+        assert torch.equal(x[:rows], want.float().to(DTYPES[dtype])) and (x[rows:] == 3).all()
+    again = ops.kv_load_fp8(*c["cache"].views, c["table"].to(device), ints(start, device), ints(c["total"], device), rows, DTYPES[dtype])
+    assert all(torch.equal(a, b[:rows]) for a, b in zip(again, got))
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+SHAPES = [(4, 1, 128, 128), (2, 2, 128, 16), (8, 1, 64, 48), (14, 2, 64, 64), (16, 1, 128, 64), (5, 1, 128, 256), (32, 1, 64, 16), (40, 1, 128, 128),
+          (2, 1, 256, 32), (3, 3, 80, 16)]
+
+
+@pytest.mark.parametrize("device", devices())
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n_q,n_kv,d,page", SHAPES)
+def test_single_tokens(n_q, n_kv, d, page, dtype, device):
+    before = [0, 1, 15, 63, 64, 200, 333] if device == "cuda" else [0, 1, 63, 70]
+    c = case([1] * len(before), before, n_q, n_kv, d, page, DTYPES[dtype], device, seed=page + n_q, stale_nan=True, ld_extra=16)
+    check_attention(run_attention(c), oracle(c), c["dtype"], d, c["n_keys"])
+
+
+@pytest.mark.parametrize("device", devices())
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n_q,n_kv,d,page", SHAPES)
+def test_chunks(n_q, n_kv, d, page, dtype, device):
+    new, before = ([3, 1, 70, 0, 17, 130, 5], [0, 40, 0, 9, 64, 61, 129]) if device == "cuda" else ([3, 1, 0, 17], [0, 40, 9, 61])
+    c = case(new, before, n_q, n_kv, d, page, DTYPES[dtype], device, seed=page + n_q, stale_nan=True, ld_extra=8, tail_rows=3)
+    out = torch.full((c["q"].shape[0], n_q * d + 24), 5.0, dtype=c["dtype"], device=device)
+    check_attention(run_attention(c, out=out), oracle(c), c["dtype"], d, c["n_keys"])
+    assert (out[-3:] == 5).all() and (out[:, n_q * d:] == 5).all()      # rows of no sequence, columns of nobody
+
+
+@pytest.mark.parametrize("device", devices())
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_rows_without_keys_are_zero(d, device):
+    """More queries than keys, and no keys at all: the first rows see nothing."""
+    c = case([4, 1, 40, 2], [0, 0, 0, 3], 4, 2, d, 16, torch.bfloat16, device, seed=3, stale_nan=False)
+    c["total"] = [2, 0, 7, 5]
+    got = run_attention(c)
+    check_attention(got, oracle(c), c["dtype"], d, 7)
+    rows = got.cpu()
+    assert (rows[:2] == 0).all() and (rows[4] == 0).all() and (rows[5: 5 + 33] == 0).all() and (rows[2:4] != 0).any()
+
+
+def test_a_step_through_store_attention_and_load():
+    """The operators together on the CPU, as a model's layer calls them: a prompt in two chunks, then single tokens."""
+    _run_together("cpu", torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_step_through_store_attention_and_load_gpu(d, dtype):
+    _run_together("cuda", DTYPES[dtype], d)
+
+
+def _run_together(device, dtype, d=64):
+    from modular_b200.nn.rotary_embedding import RopeScaling, cos_sin_table
+    n_q, n_kv, page = 4, 2, 16
+    g = torch.Generator().manual_seed(5)
+    cs = cos_sin_table(d, 128, 10000.0, RopeScaling(rope_type="llama3", factor=8.0, original_max_position_embeddings=64), device)
+    cache = Cache(8, n_kv, page, d, device)
+    table = torch.tensor([[5, 2, 7, 0]], dtype=torch.int32)
+    held = [torch.zeros(8, n_kv, page, d, dtype=torch.float64) for _ in range(2)]
+    done = 0
+    for n in (21, 9, 1, 1):
+        x = torch.randn(n, (n_q + 2 * n_kv) * d, generator=g).to(dtype)
+        pos = torch.arange(done, done + n)
+        slots = table[0].long()[pos // page] * page + pos % page
+        qkv = x.to(device)
+        q = ops.rope_kv_store_fp8(qkv, pos.int().to(device), slots.to(device), cs, *cache.views, n_q, n_kv, d)
+        a = (q, *cache.views, table.to(device), ints([0], device), ints([n], device), ints([done + n], device), n_q, n_kv, d, d ** -0.5)
+        got = ops.paged_attention_fp8(*a)
+        r = x.double().view(n, -1, d)
+        turned = rotate(r[:, : n_q + n_kv], cs.cpu().double()[pos], d, False)
+        for i, part in enumerate((turned[:, n_q:], r[:, n_q + n_kv:])):
+            y, e = quantise(part)
+            held[i][slots // page, :, slots % page] = y * 2.0 ** (e.double() - 127).unsqueeze(-1)
+        done += n
+        want = attention(q.cpu(), *held, table, [0], [n], [done], n_q, n_kv, d, d ** -0.5)
+        check_attention(got, want, dtype, d, done)
+        loaded = ops.kv_load_fp8(*cache.views, table.to(device), ints([0], device), ints([done], device), done, torch.float32)
+        for x, h in zip(loaded, held):
+            assert torch.equal(x.cpu().double(), h[table[0].long()].transpose(1, 2).reshape(-1, n_kv, d)[:done])
+
+
+# ------------------------------------------------------------------------------------------------------------ refusals
+def _args(device="cpu", d=64, page=16, n_kv=2, T=3, n_q=4, dtype=torch.bfloat16):
+    cache = Cache(4, n_kv, page, d, device)
+    qkv = torch.zeros(T, (n_q + 2 * n_kv) * d, dtype=dtype, device=device)
+    return cache, qkv, torch.zeros(4, d, device=device)
+
+
+@pytest.mark.parametrize("device", devices())
+def test_refusals(device):
+    cache, qkv, cs = _args(device)
+    pos, slots = torch.zeros(3, dtype=torch.int32, device=device), torch.arange(3, device=device)
+    k, v, ks, vs = cache.views
+    store = lambda *c, **kw: ops.rope_kv_store_fp8(qkv, pos, slots, cs, *c, 4, 2, 64, **kw)  # noqa: E731
+    errors = (ValueError, RuntimeError)
+    store(k, v, ks, vs)
+    for bad in ((k.view(torch.uint8), v, ks, vs), (k, v, ks.view(torch.int8), vs), (k, v, ks[:, :1], vs), (k[:, :1], v, ks[:, :1], vs),
+                (k[..., :48], v[..., :48], ks, vs), (k[:, :, :8], v[:, :, :8], ks[:, :, :8], vs[:, :, :8])):
+        with pytest.raises(errors):
+            store(*bad)
+    for kw in (dict(rot_dims=65), dict(rot_dims=7), dict(rot_dims=-2)):
+        with pytest.raises(errors):
+            store(k, v, ks, vs, **kw)
+    t = ints([[0, 1, 2, 3]], device)
+    one = lambda n: ints([n], device)  # noqa: E731
+    att = lambda q=qkv, scale=0.125, n_q=4, n_kv=2: ops.paged_attention_fp8(q, k, v, ks, vs, t, one(0), one(3), one(3), n_q, n_kv, 64, scale)  # noqa: E731
+    att()
+    for kw in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(n_q=3), dict(n_kv=0), dict(n_kv=1)):
+        with pytest.raises((*errors, ZeroDivisionError)):
+            att(**kw)
+    for layer in (-1, 3):
+        with pytest.raises(ValueError):
+            ops.fp8_cache_views(cache.kv, layer)
+    with pytest.raises(ValueError):
+        ops.fp8_cache_views(cache.kv.float(), 0)
+
+
+@gpu
+def test_refusals_of_layout_and_device():
+    cache, qkv, cs = _args("cuda")
+    k, v, ks, vs = cache.views
+    pos, slots = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.arange(3, device="cuda")
+    with pytest.raises(RuntimeError):                        # rows that do not start on 16 bytes
+        ops.rope_kv_store_fp8(torch.zeros(3, 516, dtype=torch.bfloat16, device="cuda")[:, 1:513], pos, slots, cs, k, v, ks, vs, 4, 2, 64)
+    with pytest.raises(RuntimeError):
+        ops.rope_kv_store_fp8(qkv, pos.cpu(), slots, cs, k, v, ks, vs, 4, 2, 64)
+    with pytest.raises(RuntimeError):
+        ops.rope_kv_store_fp8(qkv, pos, slots.int(), cs, k, v, ks, vs, 4, 2, 64)
+    with pytest.raises(RuntimeError):
+        ops.rope_kv_store_fp8(qkv, pos, slots, cs[:, :32], k, v, ks, vs, 4, 2, 64)
+    odd = torch.zeros(4 * 2 * 16 * 64 + 64, dtype=torch.uint8, device="cuda")[8: 8 + 4 * 2 * 16 * 64].view(torch.float8_e4m3fn).view(4, 2, 16, 64)
+    with pytest.raises(RuntimeError):                        # a cache that does not start on 16 bytes
+        ops.rope_kv_store_fp8(qkv, pos, slots, cs, odd, v, ks, vs, 4, 2, 64)
+    with pytest.raises(RuntimeError):
+        ops.paged_attention_fp8(qkv.int(), k, v, ks, vs, ints([[0]], "cuda"), ints([0], "cuda"), ints([3], "cuda"), ints([3], "cuda"), 4, 2, 64, 0.1)
+    with pytest.raises(RuntimeError):
+        ops.paged_attention_fp8(qkv, k, v, ks, vs, ints([[0]], "cuda"), ints([0], "cuda"), ints([3], "cuda"), ints([], "cuda"), 4, 2, 64, 0.1,
+                                plan=(None, None, None))
+
+
+@gpu
+def test_pages_slots_and_positions_out_of_range_are_reported():
+    """The kernels check them: nothing is read or written there, and the error word names it."""
+    cache, qkv, cs = _args("cuda")
+    k, v, ks, vs = cache.views
+    cache.kv.fill_(0x38)
+    one = lambda *a: ints(a, "cuda")  # noqa: E731
+    for pos, slot in (([0, 9, 1], [0, 1, 2]), ([0, -1, 1], [0, 1, 2]), ([0, 1, 2], [0, 64, 2])):
+        ops.rope_kv_store_fp8(qkv, one(*pos), torch.tensor(slot, device="cuda"), cs, k, v, ks, vs, 4, 2, 64)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError):
+            ops.check_device_error()
+    for table in ([[99]], [[-3]]):
+        for n in (1, 3):
+            ops.paged_attention_fp8(qkv[:n].contiguous(), k, v, ks, vs, ints(table, "cuda"), one(0), one(n), one(5), 4, 2, 64, 0.1)
+            torch.cuda.synchronize()
+            with pytest.raises(RuntimeError):
+                ops.check_device_error()
+    ops.paged_attention_fp8(qkv, k, v, ks, vs, ints([[0]], "cuda"), one(0), one(3), one(40), 4, 2, 64, 0.1)      # more keys than pages
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        ops.check_device_error()
+    ops.kv_load_fp8(k, v, ks, vs, ints([[77]], "cuda"), one(0), one(3), 3)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        ops.check_device_error()
