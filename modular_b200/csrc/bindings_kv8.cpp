@@ -162,7 +162,7 @@ void paged_attention_fp8(const Tensor& q, Tensor& out, const Tensor& k_cache, co
   a.err = error_flag_on(q.get_device());
   // The partial results of rows whose keys are shared out: taken from the allocator for each call, so that calls on several
   // streams and captured graphs never share them.
-  a.ws_bytes = mb_paged_attention_fp8_workspace(a.T, a.B, a.n_tiles, a.n_decode, n_q, n_kv, hd, num_sms());
+  a.ws_bytes = a.dtype == 1 ? 0 : mb_paged_attention_fp8_workspace(a.T, a.B, a.n_tiles, a.n_decode, n_q, n_kv, hd, num_sms());
   Tensor ws;
   if (a.ws_bytes > 0) {
     ws = torch::empty({static_cast<int64_t>(a.ws_bytes)}, q.options().dtype(at::kByte));

@@ -4,26 +4,19 @@
 //
 // Queries are the last q_len tokens of their sequence; a row without keys is zero.
 //
+// 16-bit queries with heads of 64 or 128 go to attention_fp8_decode.cu (sequences of up to 16 rows a head) and attention_fp8_chunk.cu; the rest to
+//
 //   attn_rows_kernel    any head width up to 256 and any group of heads, fp32 queries too: on the CUDA cores
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "../common/api.h"
 #include "../common/launch.h"
 #include "../common/ptx.cuh"
+#include "attention_fp8.cuh"
 
 namespace mb {
 namespace a8 {
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float pow2_byte(uint8_t b) { return __uint_as_float(b == 0 ? 0x400000u : static_cast<uint32_t>(b) << 23); }
-__device__ __forceinline__ float2 two_codes(uint32_t w) {
-  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3)));
-}
 
 struct RowsParams {
   MbFp8Attention a;
@@ -135,22 +128,38 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const RowsParams p) {
 
 using namespace mb;
 
-extern "C" size_t mb_paged_attention_fp8_workspace(int T, int B, int n_tiles, int n_decode, int n_q, int n_kv, int head_dim, int num_sms) {
-  (void)T; (void)B; (void)n_tiles; (void)n_decode; (void)n_q; (void)n_kv; (void)head_dim; (void)num_sms;
-  return 0;
+static bool on_tensor_cores(const MbFp8Attention& a) { return a.dtype != 1 && (a.head_dim == 64 || a.head_dim == 128) && a.n_q / a.n_kv <= 64; }
+static size_t decode_part(const MbFp8Attention& a, int num_sms) {
+  return (mb::a8::decode_workspace(a.n_decode, a.n_q, a.n_kv, a.head_dim, num_sms) + 255) / 256 * 256;
 }
 
-extern "C" int mb_paged_attention_fp8(const MbFp8Attention* a, const MbFp8Cache* c, int num_sms, cudaStream_t stream) {
+extern "C" size_t mb_paged_attention_fp8_workspace(int T, int B, int n_tiles, int n_decode, int n_q, int n_kv, int head_dim, int num_sms) {
+  MbFp8Attention a = {};
+  a.T = T; a.B = B; a.n_tiles = n_tiles; a.n_decode = n_decode; a.n_q = n_q; a.n_kv = n_kv; a.head_dim = head_dim;
+  if (T <= 0 || B <= 0 || n_kv < 1 || !on_tensor_cores(a)) return 0;
+  return decode_part(a, num_sms) + mb::a8::chunk_workspace(a, num_sms);
+}
+
+extern "C" int mb_paged_attention_fp8(const MbFp8Attention* in, const MbFp8Cache* c, int num_sms, cudaStream_t stream) {
   using namespace mb::a8;
-  (void)num_sms;
-  if (a->T <= 0 || a->B <= 0) return MB_OK;
-  if (a->n_kv < 1 || a->n_q < 1 || a->n_q % a->n_kv || a->head_dim < 16 || a->head_dim > 256 || a->head_dim % 16) return MB_ERR_SHAPE;
-  if (c->page_size < 16 || c->page_size % 16 || c->pages < 1 || !(a->scale > 0.f) || a->n_q > 65535) return MB_ERR_SHAPE;
+  MbFp8Attention a = *in;
+  if (a.T <= 0 || a.B <= 0) return MB_OK;
+  if (a.n_kv < 1 || a.n_q < 1 || a.n_q % a.n_kv || a.head_dim < 16 || a.head_dim > 256 || a.head_dim % 16 || a.dtype < 0 || a.dtype > 2) return MB_ERR_SHAPE;
+  if (c->page_size < 16 || c->page_size % 16 || c->pages < 1 || !(a.scale > 0.f) || a.n_q > 65535) return MB_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->ks) | reinterpret_cast<uintptr_t>(c->vs) |
        static_cast<uintptr_t>(c->k_page | c->k_head | c->v_page | c->v_head | c->ks_page | c->ks_head | c->vs_page | c->vs_head)) & 15)
     return MB_ERR_ALIGN;
-  if (((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15) || a->ldq % 8 || a->ldo % 8) return MB_ERR_ALIGN;
-  RowsParams p = {*a, *c};
-  auto kern = a->dtype == 0 ? attn_rows_kernel<__nv_bfloat16> : a->dtype == 1 ? attn_rows_kernel<float> : attn_rows_kernel<__half>;
-  return launch_k(kern, dim3(a->T, a->n_q), dim3(128), 0, stream, p) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
+  if (((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) || a.ldq % 8 || a.ldo % 8) return MB_ERR_ALIGN;
+  if (on_tensor_cores(a)) {
+    const size_t first = decode_part(a, num_sms);
+    if (a.ws_bytes < first) return MB_ERR_TOO_LARGE;
+    const int rc = decode_attention(a, *c, num_sms, stream);
+    if (rc != MB_OK) return rc;
+    a.ws = static_cast<char*>(a.ws) + first;
+    a.ws_bytes -= first;
+    return chunk_attention(a, *c, num_sms, stream);
+  }
+  const RowsParams p = {a, *c};
+  auto kern = a.dtype == 0 ? attn_rows_kernel<__nv_bfloat16> : a.dtype == 1 ? attn_rows_kernel<float> : attn_rows_kernel<__half>;
+  return launch_k(kern, dim3(a.T, a.n_q), dim3(128), 0, stream, p) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }

@@ -1,0 +1,79 @@
+// What the kernels of attention over the 8-bit cache share.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "../common/api.h"
+
+namespace mb {
+namespace a8 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;       // maximum of a row that has seen no key: 2^(kNoMax - anything) is zero, and nothing is infinite
+constexpr float kShift = 7.f;          // weights carry 2^7: f16 keeps 11 bits down to 2^-14 and something down to 2^-24
+// exponents of values are taken as -100 at least, which keeps 2^-e and its sums inside fp32, and as 126 at most
+constexpr int kLeastByte = 27, kMostByte = 253;
+
+__device__ __forceinline__ float pow2_byte(uint8_t b) { return __uint_as_float(b == 0 ? 0x400000u : static_cast<uint32_t>(b) << 23); }
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }      // -126 <= e <= 127
+// two e4m3 codes (the low 16 bits) as f16 pairs, exact
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3);
+  return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+}
+__device__ __forceinline__ float2 two_codes(uint32_t w) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3)));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;
+}
+// Queries go to f16 times 2^shift, which puts the largest of the tile's into [2^14, 2^15): bf16 values down to 2^-31 of it stay exact.
+__device__ __forceinline__ int f16_shift(float big) {
+  const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
+  return big > 0.f ? min(max(14 - e, -120), 120) : 0;
+}
+// x 2^e, kept inside the normal numbers: a factor of zero would make NaN of a masked score, and of a score that small nothing is left
+__device__ __forceinline__ float score_factor(float x, int e) { return fminf(fmaxf(scalbnf(x, e), 1.1754944e-38f), 8.5e37f); }
+
+// 16 consecutive values (32 bytes, 16-byte aligned)
+template <typename T>
+__device__ __forceinline__ void load16(const T* src, float (&x)[16], bool valid) {
+  uint4 r[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (valid) { r[0] = reinterpret_cast<const uint4*>(src)[0]; r[1] = reinterpret_cast<const uint4*>(src)[1]; }
+  const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float2 f;
+    if constexpr (sizeof(T) == 2 && __is_same(T, __half)) f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    x[2 * i] = f.x; x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v, float f) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x * f, v.y * f), b = __floats2bfloat162_rn(v.z * f, v.w * f);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ void store4(__half* p, float4 v, float f) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_f16(v.x * f, v.y * f), pack_f16(v.z * f, v.w * f));
+}
+
+// attention_fp8_decode.cu: the sequences of the decode list; attention_fp8_chunk.cu: the tiles. 16-bit queries, heads of 64 or 128.
+size_t decode_workspace(int n_decode, int n_q, int n_kv, int head_dim, int num_sms);
+int decode_attention(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cudaStream_t stream);
+size_t chunk_workspace(const MbFp8Attention& a, int num_sms);
+int chunk_attention(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cudaStream_t stream);
+
+}  // namespace a8
+}  // namespace mb

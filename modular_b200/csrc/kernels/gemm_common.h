@@ -15,4 +15,9 @@ int cached_tmap(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols
 int cached_tmap_raw(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
                     uint32_t box_bytes);
 
+// Rows of the 8-bit key/value cache: boxes of `box_rows` rows of `cols` bytes (64 or 128: swizzled over as many) out of a
+// [pages, heads, page, cols] byte tensor whose pages and heads lie any multiple of 16 bytes apart. Made for each call, not cached.
+int make_tmap_pages(CUtensorMap* out, const void* base, uint32_t cols, uint32_t page, uint32_t heads, uint32_t pages,
+                    uint64_t head_stride, uint64_t page_stride, uint32_t box_rows);
+
 }  // namespace mb

@@ -1292,6 +1292,20 @@ int cached_tmap_raw(CUtensorMap* out, const void* base, uint64_t rows, uint64_t 
   return MB_OK;
 }
 
+int make_tmap_pages(CUtensorMap* out, const void* base, uint32_t cols, uint32_t page, uint32_t heads, uint32_t pages,
+                    uint64_t head_stride, uint64_t page_stride, uint32_t box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return MB_ERR_DRIVER;
+  const cuuint64_t dims[4] = {cols, page, heads, pages};
+  const cuuint64_t strides[3] = {cols, head_stride, page_stride};
+  const cuuint32_t box[4] = {cols, box_rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MB_OK : MB_ERR_TMAP;
+}
+
 static uint32_t pow2_cols(int c) {
   uint32_t p = 32;
   while (static_cast<int>(p) < c) p <<= 1;
