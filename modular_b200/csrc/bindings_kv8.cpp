@@ -104,7 +104,7 @@ void rope_kv_store_fp8(const Tensor& qkv, const Tensor& positions, const Tensor&
   }
   TORCH_CHECK(T < (1ll << 31), "tokens");
   check_rc(mb_rope_kv_store_fp8(qkv.data_ptr(), ld, q_out.data_ptr(), ldq, dt, i32(positions, T, qkv, "positions"), slots.data_ptr<int64_t>(), cs,
-                                n_pos, &c, static_cast<int>(T), n_q, n_kv, hd, rot, interleaved, error_flag_on(qkv.get_device()), cur_stream()),
+                                n_pos, &c, static_cast<int>(T), n_q, n_kv, hd, rot, interleaved, error_flag_on(qkv.get_device()), num_sms(), cur_stream()),
            "rope_kv_store_fp8");
 }
 

@@ -18,10 +18,16 @@ constexpr int kLeastByte = 27, kMostByte = 253;
 
 __device__ __forceinline__ float pow2_byte(uint8_t b) { return __uint_as_float(b == 0 ? 0x400000u : static_cast<uint32_t>(b) << 23); }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }      // -126 <= e <= 127
-// two e4m3 codes (the low 16 bits) as f16 pairs, exact
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3);
-  return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+// four e4m3 codes as two pairs of f16, exact
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t"
+      ".reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t"
+      "}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 __device__ __forceinline__ float2 two_codes(uint32_t w) {
   return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3)));

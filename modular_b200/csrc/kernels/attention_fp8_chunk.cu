@@ -313,10 +313,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           const uint32_t words[4] = {c.x, c.y, c.z, c.w};
           uint32_t h[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t x = codes_f16(words[k >> 1] >> (16 * (k & 1)));
-            const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), f2);
-            h[k] = *reinterpret_cast<const uint32_t*>(&y);
+          for (int k = 0; k < 4; ++k) {
+            uint32_t x[2];
+            codes_f16(words[k], x[0], x[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), f2);
+              h[2 * k + e] = *reinterpret_cast<const uint32_t*>(&y);
+            }
           }
           uint8_t* dst = to + (chunk >> 2) * 8192 + row * 128;
           const int piece = 2 * (chunk & 3), swap = NC == 2 ? (chunk >> 2) : 0;

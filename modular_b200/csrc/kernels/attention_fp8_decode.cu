@@ -5,8 +5,8 @@
 //   * The 64-token tiles of all sequences are one line of work per head, cut into equal shares (two tiles at least) for as many CTAs
 //     as the SMs hold. A sequence inside one share is finished there; the pieces of one that is cut go to the workspace and
 //     join_kernel puts them together, in the order of the shares.
-//   * A CTA is a producer warp (TMA: K and V boxes, bulk copies of the exponents, a ring of stages) and four warps that take 16 tokens of
-//     a tile each, for all query rows (the 16 rows of one mma.sync m16n8k16, f16 operands, fp32 sums).
+//   * A CTA is a producer warp (TMA: K and V boxes, bulk copies of the exponents, a ring of stages) and two pairs of warps that take the tiles in
+//     turn, 32 tokens a warp, for all query rows (the 16 rows of one mma.sync m16n8k16, f16 operands, fp32 sums).
 //   * Codes become f16 in registers, exactly and without their scale. A lane's 16 bytes of a key are the operands of four k-steps (the order of
 //     k is free as long as the queries, loaded once, have the same). Values come through ldmatrix.trans as byte pairs, one permutation
 //     and one conversion per two values; even and odd columns are separate MMA columns.
@@ -29,8 +29,8 @@
 namespace mb {
 namespace a8 {
 
-constexpr int kDecStages = 4;
-constexpr int kDecCtas = 3;             // per SM
+constexpr int kDecStages = 6;
+constexpr int kDecCtas = 2;             // per SM
 constexpr int kMinShare = 2;            // tiles
 constexpr int kDecThreads = 160;
 constexpr int kMaxDecode = 4096;        // sequences of a launch (their tile counts wait in shared memory)
@@ -63,8 +63,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ int value_byte(uint8_t b) { return min(max(static_cast<int>(b), kLeastByte), kMostByte); }
-
 // tiles of sequence i of the decode list
 __device__ __forceinline__ int tiles_of(const MbFp8Attention& a, int i) {
   const int seq = a.decode_seq[i];
@@ -79,6 +77,134 @@ __device__ __forceinline__ int share_holding(int U, int G, int u) { return stati
 // A partial result: fp32 O [rows][HD], then m [16], l [16]; two slots per CTA (its first and its last sequence)
 template <int HD>
 __host__ __device__ constexpr int slot_floats(int rows) { return rows * HD + 32; }
+
+// Rows g and g + 8 of a warp's state, columns 16 c + 4 t4 + {0, 2} of the even and {1, 3} of the odd MMA columns of chunk c
+template <int HD>
+struct RowState {
+  float o[HD / 8][4];
+  float m[2], l[2];
+};
+
+// Token order inside a group of 8: with 128-byte rows tokens 0, 4, 1, 5, .. alternate between the halves of the swizzle, so that the eight lanes
+// of a quarter-warp read from all banks.
+template <int HD>
+__device__ __forceinline__ int order(int n) { return HD == 128 ? (n >> 1) + (n & 1) * 4 : n; }
+
+// 32 tokens from key k0 on, rows row0 and up of the tile. sE: exponent bytes of the keys, those of the values 64 bytes behind. Four groups of eight
+// tokens side by side: one group's products wait for one another.
+template <int HD, bool EDGE>
+__device__ __forceinline__ void walk32(RowState<HD>& st, const uint32_t (&qf)[HD / 16][4], uint32_t sK, uint32_t sV, uint32_t sE, float sc, int row0,
+                                       int lane, int k0, int kl, const int (&limit)[2]) {
+  const int g = lane >> 2, t4 = lane & 3;
+  // ---- scores of 4 x 8 tokens
+  float c[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+#pragma unroll
+  for (int n = 0; n < HD / 64; ++n) {
+    uint4 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = row0 + j * 8 + order<HD>(g), chunk = n * 4 + t4;
+      w[j] = lds128(sK + (HD == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t lo, hi;
+        codes_f16(k == 0 ? w[j].x : k == 1 ? w[j].y : k == 2 ? w[j].z : w[j].w, lo, hi);
+        mma_f16(c[j], qf[n * 4 + k], lo, hi);
+      }
+  }
+  // ---- weights: column 2 t4 + e of group j is token 8 j + order(2 t4 + e). Its byte becomes a float's exponent (the scale of K), a float (the
+  // exponent of V, as the low bits of 2^23) and an exponent again (the way back).
+  float back[4][2];
+  bool grow = false;
+  float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {
+    const uint4 kb4 = lds128(sE + jj * 16), vb4 = lds128(sE + 64 + jj * 16);
+    const uint32_t kb[4] = {kb4.x, kb4.y, kb4.z, kb4.w}, vb[4] = {vb4.x, vb4.y, vb4.z, vb4.w};
+#pragma unroll
+    for (int j2 = 0; j2 < 2; ++j2)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = jj * 2 + j2, tok = j * 8 + order<HD>(2 * t4 + e);
+        // HD 128: tokens t4, 4 + t4 of group j, byte t4 of a word each; HD 64: tokens 2 t4 and 2 t4 + 1
+        const uint32_t sel = HD == 128 ? t4 : 2 * (t4 & 1) + e;
+        const uint32_t kw = HD == 128 ? kb[2 * j2 + e] : (t4 < 2 ? kb[2 * j2] : kb[2 * j2 + 1]);
+        const uint32_t vw = HD == 128 ? vb[2 * j2 + e] : (t4 < 2 ? vb[2 * j2] : vb[2 * j2 + 1]);
+        const float ak = __uint_as_float(__byte_perm(kw, 0, 0x4440 | sel) << 23) * sc;
+        const uint32_t vbyte = __byte_perm(vw, 0x4B000000u, 0x7440 | sel);       // 2^23 + byte
+        const float ev = fmaxf(__uint_as_float(vbyte) - 8388735.f, -100.f);
+        back[j][e] = fminf(__uint_as_float((0x4B0000FEu - vbyte) << 23), 1.2676506e30f);        // 2^-ev, 2^100 at most
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x = fmaf(c[j][2 * h + e], ak, ev);
+          if (EDGE) x = k0 + tok <= limit[h] ? x : -INFINITY;
+          c[j][2 * h + e] = x;
+          top[h] = fmaxf(top[h], x);
+        }
+      }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) grow |= top[h] > st.m[h] + 8.f;
+  if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(st.m[h], mx), f = exp2f(st.m[h] - mn);
+      st.m[h] = mn;
+      st.l[h] *= f;
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) { st.o[d][2 * h] *= f; st.o[d][2 * h + 1] *= f; }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float ref = st.m[h] - kShift;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float pv = ex2(c[j][2 * h + e] - ref);
+        c[j][2 * h + e] = pv;
+        // (the byte of a key that is not there may be anything)
+        st.l[h] = fmaf(pv, EDGE && pv == 0.f ? 0.f : back[j][e], st.l[h]);
+      }
+  }
+  // ---- values. Rows behind the last key are zeroed: they may hold anything, NaN among it
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {
+    const uint32_t pa[4] = {pack_f16(c[2 * jj][0], c[2 * jj][1]), pack_f16(c[2 * jj][2], c[2 * jj][3]), pack_f16(c[2 * jj + 1][0], c[2 * jj + 1][1]),
+                            pack_f16(c[2 * jj + 1][2], c[2 * jj + 1][3])};
+    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+    if (EDGE) {
+      const int valid = kl - k0 - jj * 16;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        keep[j] = (j * 8 + order<HD>(2 * t4) < valid ? 0xffffu : 0u) | (j * 8 + order<HD>(2 * t4 + 1) < valid ? 0xffff0000u : 0u);
+    }
+    const int row = row0 + jj * 16 + ((lane >> 3) & 1) * 8 + order<HD>(lane & 7);
+#pragma unroll
+    for (int cp = 0; cp < HD / 32; ++cp) {
+      const int chunk = 2 * cp + (lane >> 4);
+      uint32_t r[4];
+      ldsm_x4_t(r, sV + (HD == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)));
+      if (EDGE) { r[0] &= keep[0]; r[1] &= keep[1]; r[2] &= keep[0]; r[3] &= keep[1]; }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t even[2], odd[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) codes_f16(__byte_perm(r[2 * k + j], 0, 0x3120), even[j], odd[j]);
+        mma_f16(st.o[(2 * cp + k) * 2], pa, even[0], even[1]);
+        mma_f16(st.o[(2 * cp + k) * 2 + 1], pa, odd[0], odd[1]);
+      }
+    }
+  }
+}
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(kDecThreads, kDecCtas)
@@ -98,7 +224,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.y, nd = p.a.n_decode, G = p.a.n_q / p.a.n_kv;
   if (tid == 0) {
-    for (int s = 0; s < kDecStages; ++s) { mbar_init(&bars.full[s], 1); mbar_init(&bars.empty[s], 4); }
+    for (int s = 0; s < kDecStages; ++s) { mbar_init(&bars.full[s], 1); mbar_init(&bars.empty[s], 2); }
     bars.abort_word = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
@@ -201,13 +327,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
     return;
   }
 
-  // ------------------------------------------------------------------ four warps of 16 tokens a tile
+  // ------------------------------------------------------------------ two pairs of warps take tiles in turn, 32 tokens a warp
   const int g = lane >> 2, t4 = lane & 3;
-  // token order inside a group of 8: with 128-byte rows tokens 0, 4, 1, 5, .. alternate between the halves of the swizzle, so that the eight lanes of
-  // a quarter-warp read from all banks
-  auto order = [](int n) { return HD == 128 ? (n >> 1) + (n & 1) * 4 : n; };
-  const int ka = order(g), va = order(lane & 7);
-  int s = 0;
+  int s = 0, turn = 0;
   uint32_t ph = 0;
   bool ok = true;
   for (int i = first, u = u0; u < u1; ++i) {
@@ -247,114 +369,40 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
         qf[n * 4 + k][3] = pack_f16(qv[1][n][4 * k + 2] * qmul, qv[1][n][4 * k + 3] * qmul);
       }
     const float sc = score_factor(p.a.scale * kLog2e, -qe);
-    float o[HD / 8][4];
+    RowState<HD> st;
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
-    float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+    for (int d = 0; d < HD / 8; ++d) st.o[d][0] = st.o[d][1] = st.o[d][2] = st.o[d][3] = 0.f;
+    st.m[0] = st.m[1] = kNoMax;
+    st.l[0] = st.l[1] = 0.f;
     int limit[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) limit[h] = g + 8 * h < rows ? kl - ql + (g + 8 * h) / G : -1;
 
-    for (int t = ta; t < tb && ok; ++t) {
-      // (after a failed wait a warp skips the remaining tiles but meets the others at every barrier)
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars.full[s], ph, abort_word, p.a.err, 742));
-      if (!ok) break;
-      const int k0 = t * 64 + warp * 16;            // first of this warp's tokens
-      if (k0 < kl) {
-        const uint32_t sK = smem_u32(smem + s * kStage), sV = sK + kCodes;
-        const uint8_t* bytes = sScale + s * 128 + warp * 16;
-        // ---- scores of 2 x 8 tokens
-        float c[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-          const int row = warp * 16 + j * 8 + ka;
-#pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            const int chunk = n * 4 + t4;
-            const uint4 w = lds128(sK + (HD == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)));
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f16(c[j], qf[n * 4 + k], codes_f16(ws[k]), codes_f16(ws[k] >> 16));
-          }
-        }
-        // ---- weights: column 2 t4 + e of group j is token 8 j + order(2 t4 + e)
-        float w[2][2][2];                           // [row half][j][e]
-        float grow = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int tok = j * 8 + order(2 * t4 + e), key = k0 + tok;
-            const float ak = __uint_as_float(static_cast<uint32_t>(bytes[tok]) << 23) * sc, ev = static_cast<float>(value_byte(bytes[64 + tok]) - 127);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float x = key <= limit[h] ? fmaf(c[j][2 * h + e], ak, ev) : -INFINITY;
-              w[h][j][e] = x;
-              if (x > m[h] + 8.f) grow = 1.f;
-            }
-          }
-        if (__any_sync(0xffffffffu, grow != 0.f)) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(fmaxf(w[h][0][0], w[h][0][1]), fmaxf(w[h][1][0], w[h][1][1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[h], mx), f = exp2f(m[h] - mn);
-            m[h] = mn;
-            l[h] *= f;
-#pragma unroll
-            for (int d = 0; d < HD / 8; ++d) { o[d][2 * h] *= f; o[d][2 * h + 1] *= f; }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int tok = j * 8 + order(2 * t4 + e);
-            const float back = __uint_as_float(static_cast<uint32_t>(254 - value_byte(bytes[64 + tok])) << 23);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float pv = ex2(w[h][j][e] - (m[h] - kShift));
-              w[h][j][e] = pv;
-              l[h] = fmaf(pv, back, l[h]);
-            }
-          }
-        const uint32_t pa[4] = {pack_f16(w[0][0][0], w[0][0][1]), pack_f16(w[1][0][0], w[1][0][1]), pack_f16(w[0][1][0], w[0][1][1]),
-                                pack_f16(w[1][1][0], w[1][1][1])};
-        // ---- values: rows behind the last key are zeroed (they may hold anything, NaN among it)
-        const int valid = kl - k0;
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (valid < 16) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            keep[j] = (j * 8 + order(2 * t4) < valid ? 0xffffu : 0u) | (j * 8 + order(2 * t4 + 1) < valid ? 0xffff0000u : 0u);
-        }
-        const int vrow = warp * 16 + ((lane >> 3) & 1) * 8 + va;
-#pragma unroll
-        for (int cp = 0; cp < HD / 32; ++cp) {
-          const int chunk = 2 * cp + (lane >> 4);
-          uint32_t r[4];
-          ldsm_x4_t(r, sV + (HD == 128 ? vrow * 128 + ((chunk ^ (vrow & 7)) << 4) : vrow * 64 + ((chunk ^ ((vrow >> 1) & 3)) << 4)));
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t x0 = __byte_perm(r[2 * k] & keep[0], 0, 0x3120), x1 = __byte_perm(r[2 * k + 1] & keep[1], 0, 0x3120);
-            mma_f16(o[(2 * cp + k) * 2], pa, codes_f16(x0), codes_f16(x1));
-            mma_f16(o[(2 * cp + k) * 2 + 1], pa, codes_f16(x0 >> 16), codes_f16(x1 >> 16));
-          }
+    for (int t = ta; t < tb; ++t) {
+      const bool mine = turn == warp >> 1;
+      turn ^= 1;
+      if (mine && ok) {
+        // (after a failed wait a warp skips the remaining tiles but meets the others at every barrier)
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.full[s], ph, abort_word, p.a.err, 742));
+        if (ok) {
+          const int row0 = (warp & 1) * 32, k0 = t * 64 + row0;     // first of this warp's tokens
+          const uint32_t sK = smem_u32(smem + s * kStage), sV = sK + kCodes, sE = smem_u32(sScale + s * 128 + row0);
+          // the last tokens of a sequence are masked row by row; before them every row sees all
+          if (k0 + 32 <= kl - ql + 1) walk32<HD, false>(st, qf, sK, sV, sE, sc, row0, lane, k0, kl, limit);
+          else if (k0 < kl) walk32<HD, true>(st, qf, sK, sV, sE, sc, row0, lane, k0, kl, limit);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.empty[s]);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.empty[s]);
       if (++s == kDecStages) { s = 0; ph ^= 1; }
     }
 
     // ---- the four warps' states become one, in the order of the warps
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (t4 == 0) { sML[warp * 32 + g + 8 * h] = m[h]; sML[warp * 32 + 16 + g + 8 * h] = l[h]; }
+      st.l[h] += __shfl_xor_sync(0xffffffffu, st.l[h], 1);
+      st.l[h] += __shfl_xor_sync(0xffffffffu, st.l[h], 2);
+      if (t4 == 0) { sML[warp * 32 + g + 8 * h] = st.m[h]; sML[warp * 32 + 16 + g + 8 * h] = st.l[h]; }
     }
     consumers_sync();
     float f[2];
@@ -363,7 +411,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
       float top = kNoMax;
 #pragma unroll
       for (int w = 0; w < 4; ++w) top = fmaxf(top, sML[w * 32 + g + 8 * h]);
-      f[h] = exp2f(m[h] - top);
+      f[h] = exp2f(st.m[h] - top);
     }
     for (int w = 0; w < 4; ++w) {
       if (warp == w) {
@@ -374,10 +422,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
             for (int c = 0; c < HD / 16; ++c) {
               float4* at = reinterpret_cast<float4*>(sO + (g + 8 * h) * (HD + 4) + c * 16 + t4 * 4);
               float4 v = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
-              v.x = fmaf(o[2 * c][2 * h], f[h], v.x);
-              v.y = fmaf(o[2 * c + 1][2 * h], f[h], v.y);
-              v.z = fmaf(o[2 * c][2 * h + 1], f[h], v.z);
-              v.w = fmaf(o[2 * c + 1][2 * h + 1], f[h], v.w);
+              v.x = fmaf(st.o[2 * c][2 * h], f[h], v.x);
+              v.y = fmaf(st.o[2 * c + 1][2 * h], f[h], v.y);
+              v.z = fmaf(st.o[2 * c][2 * h + 1], f[h], v.z);
+              v.w = fmaf(st.o[2 * c + 1][2 * h + 1], f[h], v.w);
               *at = v;
             }
           }

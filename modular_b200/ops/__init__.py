@@ -432,7 +432,7 @@ def rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale,
     ``rot_dims`` (default head_dim, 0: no rotation) columns of a head turn, in pairs ``rot_dims / 2`` apart or neighbouring
     (``interleaved``). ``slots`` int64 [T]: page * page_size + offset, negative: the token is not stored. Two tokens of a call must not
     name one slot. The rotated queries replace those in ``qkv``, or go to ``q_out`` (then ``qkv`` stays as it is); they are returned
-    as [T, n_q * head_dim]. Rows are rounded once, from the rotation's exact result. A position or slot out of range is reported by
+    as [T, n_q * head_dim], rotated in fp32 and rounded once; the codes are those of the exact rotation. A position or slot out of range is reported by
     :func:`check_device_error` and its row is not rotated or not stored."""
     rot = head_dim if rot_dims is None else int(rot_dims)
     if rot % 2 or not 0 <= rot <= head_dim:
