@@ -53,18 +53,27 @@ __device__ __forceinline__ int f16_shift(float big) {
 // x 2^e, kept inside the normal numbers: a factor of zero would make NaN of a masked score, and of a score that small nothing is left
 __device__ __forceinline__ float score_factor(float x, int e) { return fminf(fmaxf(scalbnf(x, e), 1.1754944e-38f), 8.5e37f); }
 
+// eight 16-bit values
+template <typename T>
+__device__ __forceinline__ void widen8(uint4 r, float (&x)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f;
+    if constexpr (__is_same(T, __half)) f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    x[2 * i] = f.x; x[2 * i + 1] = f.y;
+  }
+}
 // 16 consecutive values (32 bytes, 16-byte aligned)
 template <typename T>
 __device__ __forceinline__ void load16(const T* src, float (&x)[16], bool valid) {
-  uint4 r[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  if (valid) { r[0] = reinterpret_cast<const uint4*>(src)[0]; r[1] = reinterpret_cast<const uint4*>(src)[1]; }
-  const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float2 f;
-    if constexpr (sizeof(T) == 2 && __is_same(T, __half)) f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-    x[2 * i] = f.x; x[2 * i + 1] = f.y;
+  for (int i = 0; i < 2; ++i) {
+    float y[8];
+    widen8<T>(valid ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0), y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[8 * i + k] = y[k];
   }
 }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v, float f) {

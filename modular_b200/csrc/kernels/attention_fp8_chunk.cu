@@ -1,14 +1,17 @@
 // Attention of chunks of new tokens over the 8-bit paged cache, on the 5th-generation tensor cores.
 //
-// A CTA takes 256 query rows of one (sequence, key/value head): two MMA tiles of 128, tokens x the query heads that share the head. It walks
-// the keys 64 at a time; with few CTAs the keys are shared out over grid.z and a second kernel joins the parts.
+// A segment is 256 query rows of one (sequence, key/value head): two MMA tiles of 128, tokens x the query heads that share the head, against the keys they
+// see, 64 at a time. All segments are one line of work (their tiles, and two units each for what a segment costs besides), cut into equal shares for one
+// CTA per SM. A segment that is cut leaves partial results, which join_chunks_kernel adds up.
 //
+//   warp 2        walks over the share and hands its pieces to the others
 //   warp 0        producer: codes and exponents of 64 tokens (bulk copies, the rows of a page and head lie together) into a ring
 //   warps 12-15   codes to f16, into operand tiles with the 128-byte swizzle. Within a tile a row's scale is applied relative to the largest
 //                 of the tile (a power of two: exact unless it is 2^-20 of that), so the tile has one scale left over, for K and for V
 //   warp 1        MMA issuer: S_g = Q_g . K^T of the next keys into the other of two buffers, then O_g += P_g . V (P from TMEM)
 //   warps 4-11    softmax, a query row per thread (as attention_tc.cu). The tile's scale of K is part of the score's factor; that of V, 2^E, goes
-//                 into the exponent, 2^(t + E - m), and the denominator adds the tile's sum times 2^-E
+//                 into the exponent, 2^(t + E - m), and the denominator adds the tile's sum times 2^-E. The next segment's queries are brought in
+//                 before the results of this one are read
 //
 // The MMAs of 64 keys take 1024 cycles, the exponentials as many, the conversion 16 K codes; all operands pass through shared memory.
 #include <cuda.h>
@@ -27,26 +30,43 @@ namespace a8 {
 
 constexpr int kRing = 3;                // stages of codes
 constexpr int kThreads = 512;
-constexpr int kMaxSplits = 16;
 constexpr int kHeadroom = 6;            // the tile's largest scale becomes 2^6: codes reach 2^15 of f16
+constexpr int kSetup = 2;               // units of a segment besides its tiles
+constexpr int kMinUnits = 6;            // of a share
+constexpr int kMaxTiles = 8192;         // plan tiles of a launch (their sums wait in shared memory)
 
 struct ChunkParams {
   MbFp8Attention a;
   MbFp8Cache c;
-  float* ws;                            // [split][T * n_q][HD + 2]: O, m, l
-  int splits, box;
+  float* ws;                            // [CTA][2][256][HD + 4]: O, m, l of a segment's piece that begins / ends a share
+  int* sums;                            // [n_tiles + 1], for join_chunks_kernel
+  int box;
 };
 
 struct TileInfo {
-  float k, v;                           // factor of a score, exponent of the values
+  int k;                                // exponents left over
+  float v;
 };
+// Tiles [ta, tb) of a segment's nt, as warp 2 hands them out
+struct Piece {
+  int nt, ta, tb, head;                 // nt < 0: no more
+  int seq, tq0, half_tok, two;          // two: the second MMA tile has rows
+  int qs, ql, kl, kv_hi;
+};
+constexpr int kPieces = 4;
+constexpr int kRoles = 14;              // warps that take them: producer, MMA issuer, four converters, eight of softmax
+
 struct ChunkBars {
   uint64_t full[kRing], empty[kRing];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t info_full[4];
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_done[2];       // [query tile][buffer]
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];                   // [query tile][buffer]
+  uint64_t q_full[2], o_done[2], o_free[2];
+  uint64_t piece_full[kPieces], piece_empty[kPieces];
+  Piece piece[kPieces];
   TileInfo info[4];
-  uint32_t qmax;
+  int rows[kRing];                      // keys of a tile
+  int warp_sum[kThreads / 32];
   uint32_t tmem_base;
   int abort_word;
 };
@@ -89,24 +109,59 @@ __device__ __forceinline__ uint32_t pow2_f16x2(int x) {
   return h | (h << 16);
 }
 
-// What a CTA works on. Plan tiles hold 64 / G tokens; a CTA takes up to four of them in a row.
+// A segment of the plan. Plan tiles hold 64 / G tokens; a segment takes up to four of them, the first at a multiple of four.
 struct Work {
-  int seq, tq0, qs, ql, kl, tok, last_tq, kv_hi;
+  int seq, tq0, qs, ql, kl, half_tok, kv_hi;
+  bool two;                                          // the second MMA tile has rows
 };
-__device__ __forceinline__ bool work_of(const MbFp8Attention& a, int at, Work& w) {
-  const int G = a.n_q / a.n_kv, n = a.n_tiles, lead = (n + 3) >> 2;
-  // first the tiles that surely have work (where a sequence begins at a multiple of four), later ones of a prompt, which see more keys, first
-  const int k = at - lead, tile = at < lead ? 4 * (lead - 1 - at) : k / 3 * 4 + k % 3 + 1;
-  w.tok = 64 / G;
+__device__ __forceinline__ bool work_of(const MbFp8Attention& a, int tile, Work& w) {
+  const int G = a.n_q / a.n_kv, tok = 64 / G;
   w.seq = a.tile_seq[tile];
   if (w.seq < 0) return false;
   w.tq0 = a.tile_q0[tile];
-  if (w.tq0 % (4 * w.tok) != 0) return false;       // covered by the CTA of a tile before it
+  if (w.tq0 % (4 * tok) != 0) return false;          // part of the segment of a tile before it
   w.qs = a.q_start[w.seq]; w.ql = a.q_len[w.seq]; w.kl = a.kv_len[w.seq];
-  w.last_tq = min(w.tq0 + 4 * w.tok, w.ql);
-  w.kv_hi = max(0, min(w.kl, w.kl - w.ql + w.last_tq));
+  w.half_tok = 2 * tok;
+  w.two = w.tq0 + w.half_tok < w.ql;
+  w.kv_hi = max(0, min(w.kl, w.kl - w.ql + min(w.tq0 + 4 * tok, w.ql)));
   return w.tq0 < w.ql;
 }
+
+// CTAs that get work, and the first unit of CTA c's share; U < 2^31
+__device__ __forceinline__ int chunk_shares(int64_t U, int ctas) { return static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(ctas), U / kMinUnits))); }
+__device__ __forceinline__ int64_t chunk_start(int64_t U, int C, int c) { return U * c / C; }
+__device__ __forceinline__ int chunk_holding(int64_t U, int C, int64_t u) { return static_cast<int>(((u + 1) * C - 1) / U); }
+// the tile whose units hold v: the last one whose sum is at most v
+__device__ __forceinline__ int tile_holding(const int* sums, int n, int v) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (sums[m] <= v) lo = m; else hi = m - 1;
+  }
+  return lo;
+}
+
+// The pieces of a CTA's share, in order
+struct Pieces {
+  int64_t u, end;
+  int head, tile, nt, ta, tb;
+  __device__ __forceinline__ bool next(const int* sums, int n) {
+    const int per_head = sums[n];
+    while (u < end) {
+      head = static_cast<int>(u / per_head);
+      const int v = static_cast<int>(u - static_cast<int64_t>(head) * per_head);
+      tile = tile_holding(sums, n, v);
+      const int a = v - sums[tile], len = sums[tile + 1] - sums[tile];
+      const int b = static_cast<int>(min(static_cast<int64_t>(len), a + (end - u)));
+      u += b - a;
+      nt = len - kSetup;
+      ta = max(0, a - kSetup);
+      tb = max(0, b - kSetup);
+      if (tb > ta || (nt == 0 && a == 0)) return true;       // (a share may begin or end within the units besides the tiles)
+    }
+    return false;
+  }
+};
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ ChunkParams p) {
@@ -123,16 +178,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   uint8_t* sRing = sV + 2 * Sh::kTile16;            // [stage][K codes | V codes]
   uint8_t* sScale = sRing + kRing * Sh::kStage;     // [stage][K 64 | V 64]
   ChunkBars* bars = reinterpret_cast<ChunkBars*>(sScale + kRing * 128);
+  int* sums = reinterpret_cast<int*>(bars + 1);     // [n_tiles + 1]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.x, G = p.a.n_q / p.a.n_kv;
-  pdl_wait();
-  Work w;
-  if (!work_of(p.a, blockIdx.y, w)) return;
-  const int half_tok = 2 * w.tok;                   // tokens of an MMA tile
-  const bool two = w.tq0 + half_tok < w.ql;
-  const int all_tiles = (w.kv_hi + 63) / 64;
-  const int t0 = static_cast<int>(static_cast<int64_t>(all_tiles) * blockIdx.z / p.splits);
-  const int nt = static_cast<int>(static_cast<int64_t>(all_tiles) * (blockIdx.z + 1) / p.splits) - t0;
+  const int G = p.a.n_q / p.a.n_kv, n_tiles = p.a.n_tiles;
 
   if (tid == 0) {
     for (int s = 0; s < kRing; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 4); }
@@ -140,10 +188,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       mbar_init(&bars->k_full[b], 4); mbar_init(&bars->k_empty[b], 1);
       mbar_init(&bars->v_full[b], 4); mbar_init(&bars->v_empty[b], 1);
       for (int g = 0; g < 2; ++g) { mbar_init(&bars->s_full[g][b], 1); mbar_init(&bars->p_full[g][b], 4); mbar_init(&bars->pv_done[g][b], 1); }
-      mbar_init(&bars->o_done[b], 1);
+      mbar_init(&bars->q_full[b], 4); mbar_init(&bars->o_done[b], 1); mbar_init(&bars->o_free[b], 4);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bars->info_full[i], 1);
-    bars->qmax = 0;
+    for (int i = 0; i < kPieces; ++i) { mbar_init(&bars->piece_full[i], 1); mbar_init(&bars->piece_empty[i], kRoles); }
     bars->abort_word = 0;
     fence_mbar_init();
   }
@@ -151,295 +199,429 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
-  __syncthreads();
-  // query rows: the largest value first, then f16 with the 128-byte swizzle; a thread takes its own row
-  const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
-  const int tq = w.tq0 + g * half_tok + r / G, head = kvh * G + r % G;
-  const bool softmax_warp = warp >= 4 && warp < 12;
-  const bool valid = softmax_warp && r < half_tok * G && tq < w.ql && w.qs + tq < p.a.T;
-  const T* src = static_cast<const T*>(p.a.q) + static_cast<int64_t>(valid ? w.qs + tq : 0) * p.a.ldq + static_cast<int64_t>(head) * HD;
-  if (softmax_warp) {
-    float big = 0.f;
+  pdl_wait();
+  int run = 0;                                      // running sums of the segments' units
+  for (int base = 0; base < n_tiles; base += kThreads) {
+    const int i = base + tid;
+    Work w;
+    int v = i < n_tiles && work_of(p.a, i, w) ? (w.kv_hi + 63) / 64 + kSetup : 0;
+    const int mine = v;
 #pragma unroll
-    for (int c = 0; c < HD; c += 16) {
-      float x[16];
-      load16(src + c, x, valid);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) big = fmaxf(big, finite_abs(x[k]));
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += x;
     }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-    if (lane == 0) atomicMax(&bars->qmax, top);
+    if (lane == 31) bars->warp_sum[warp] = v;
+    __syncthreads();
+    int before = run;
+    for (int k = 0; k < warp; ++k) before += bars->warp_sum[k];
+    if (i < n_tiles) sums[i] = before + v - mine;
+    for (int k = 0; k < kThreads / 32; ++k) run += bars->warp_sum[k];
+    __syncthreads();
   }
-  __syncthreads();
-  const int qe = f16_shift(__uint_as_float(bars->qmax));
-  if (softmax_warp) {
-    const float mul = pow2f(qe);
-#pragma unroll
-    for (int c = 0; c < HD; c += 16) {
-      float x[16];
-      load16(src + c, x, valid);
-      uint32_t h[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) h[k] = pack_f16(x[2 * k] * mul, x[2 * k + 1] * mul);
-      uint8_t* row = sQ + g * Sh::kQTile + (c >> 6) * 16384 + r * 128;
-      const int piece = (c & 63) >> 3;
-      *reinterpret_cast<uint4*>(row + ((piece ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint4*>(row + (((piece + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-    }
-    fence_proxy_async_smem();
-  }
+  if (tid == 0) sums[n_tiles] = run;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= n_tiles; i += kThreads) p.sums[i] = sums[i];
   const uint32_t tmem_base = bars->tmem_base;
   volatile int* abort_word = &bars->abort_word;
+  const int64_t U = static_cast<int64_t>(run) * p.a.n_kv;
+  const int C = chunk_shares(U, gridDim.x), cta = blockIdx.x;
 
   // 512 x 128 registers at launch = 128 x (48 + 192 + 192 + 80)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == 0 && lane == 0) {
-      // ---------------------------------------------------------------- producer
-      const int32_t* bt = p.a.block_table + static_cast<int64_t>(w.seq) * p.a.bt_stride;
+    if (warp == 2 && lane == 0) {
+      // ---------------------------------------------------------------- pieces
+      Pieces pc;
+      pc.u = cta < C ? chunk_start(U, C, cta) : 0;
+      pc.end = cta < C ? chunk_start(U, C, cta + 1) : 0;
+      bool more = true;
+      for (int i = 0; more; ++i) {
+        more = pc.next(sums, n_tiles);
+        Piece q;
+        q.nt = -1;
+        if (more) {
+          Work w;
+          work_of(p.a, pc.tile, w);
+          q.nt = pc.nt; q.ta = pc.ta; q.tb = pc.tb; q.head = pc.head;
+          q.seq = w.seq; q.tq0 = w.tq0; q.half_tok = w.half_tok; q.two = w.two ? 1 : 0;
+          q.qs = w.qs; q.ql = w.ql; q.kl = w.kl; q.kv_hi = w.kv_hi;
+        }
+        if (!mbar_wait(&bars->piece_empty[i % kPieces], ((i / kPieces) & 1) ^ 1, abort_word, p.a.err, 764)) break;
+        bars->piece[i % kPieces] = q;
+        mbar_arrive(&bars->piece_full[i % kPieces]);
+      }
+    } else if (warp == 0) {
+      // ---------------------------------------------------------------- producer: places of the next 32 boxes by lane, a copy per lane
+      // (one lane alone took 3250 cycles a tile, for the page number's round trip, the divisions and four copies)
+      const int per = 64 / p.box;
+      const bool is_v = lane & 1, is_exp = lane & 2;
+      const uint8_t* base = is_exp ? (is_v ? p.c.vs : p.c.ks) : static_cast<const uint8_t*>(is_v ? p.c.v : p.c.k);
+      const int64_t page_step = is_exp ? (is_v ? p.c.vs_page : p.c.ks_page) : (is_v ? p.c.v_page : p.c.k_page);
+      const int64_t head_step = is_exp ? (is_v ? p.c.vs_head : p.c.ks_head) : (is_v ? p.c.v_head : p.c.k_head);
+      const int row_bytes = is_exp ? 1 : HD;
+      uint8_t* to = (is_exp ? sScale + (is_v ? 64 : 0) : sRing + (is_v ? Sh::kCodes : 0)) + (lane >> 2) * p.box * row_bytes;
+      const int to_step = is_exp ? 128 : Sh::kStage;
       int s = 0;
       uint32_t ph = 0;
-      for (int t = 0; t < nt; ++t) {
-        const int kv0 = (t0 + t) * 64, boxes = (min(64, w.kv_hi - kv0) + p.box - 1) / p.box;
-        int page[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          page[b] = 0;
-          if (b >= boxes) continue;
-          const int nth = (kv0 + b * p.box) / p.c.page_size;
-          page[b] = nth < p.a.bt_stride ? bt[nth] : -1;
-          if (page[b] < 0 || page[b] >= p.c.pages) {               // reported; some page stands in for it
-            if (p.a.err) atomicCAS(p.a.err, 0, 731);
-            page[b] = 0;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->piece_full[i % kPieces], (i / kPieces) & 1, abort_word, p.a.err, 765));
+        if (!ok) break;
+        const Piece& q = bars->piece[i % kPieces];
+        const int ta = q.ta, tb = q.nt < 0 ? -1 : q.tb, kv_hi = q.kv_hi;
+        const uint8_t* from = base + q.head * head_step;
+        const int32_t* bt = p.a.block_table + static_cast<int64_t>(q.seq) * p.a.bt_stride;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->piece_empty[i % kPieces]);
+        if (tb < 0) break;
+        int page = 0, off = 0, at = 32;
+        for (int t = ta; t < tb; ++t, at += per) {
+          if (at == 32) {
+            at = 0;
+            const int tok = t * 64 + lane * p.box, nth = tok / p.c.page_size;
+            off = tok - nth * p.c.page_size;
+            page = 0;
+            if (tok < kv_hi) {
+              page = nth < p.a.bt_stride ? bt[nth] : -1;
+              if (page < 0 || page >= p.c.pages) {                 // reported; some page stands in for it
+                if (p.a.err) atomicCAS(p.a.err, 0, 731);
+                page = 0;
+              }
+            }
           }
+          const int n = min(64, kv_hi - t * 64), boxes = (n + p.box - 1) / p.box;
+          const int mine = min(at + (lane >> 2), 31), my_page = __shfl_sync(0xffffffffu, page, mine), my_off = __shfl_sync(0xffffffffu, off, mine);
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[s], ph ^ 1, abort_word, p.a.err, 751));
+          if (!ok) break;
+          if (lane == 0) {
+            bars->rows[s] = n;
+            mbar_arrive_expect_tx(&bars->full[s], static_cast<uint32_t>(boxes) * p.box * (2 * HD + 2));
+          }
+          __syncwarp();
+          if (lane < boxes * 4) bulk_load(to + s * to_step, from + my_page * page_step + my_off * row_bytes, p.box * row_bytes, &bars->full[s]);
+          if (++s == kRing) { s = 0; ph ^= 1; }
         }
-        if (!mbar_wait(&bars->empty[s], ph ^ 1, abort_word, p.a.err, 751)) break;
-        mbar_arrive_expect_tx(&bars->full[s], static_cast<uint32_t>(boxes) * p.box * (2 * HD + 2));
-        uint8_t* dst = sRing + s * Sh::kStage;
-        uint8_t* sc = sScale + s * 128;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (b >= boxes) continue;
-          const int64_t pg = page[b], off = (kv0 + b * p.box) % p.c.page_size;
-          bulk_load(dst + b * p.box * HD, static_cast<const uint8_t*>(p.c.k) + pg * p.c.k_page + kvh * p.c.k_head + off * HD, p.box * HD, &bars->full[s]);
-          bulk_load(dst + Sh::kCodes + b * p.box * HD, static_cast<const uint8_t*>(p.c.v) + pg * p.c.v_page + kvh * p.c.v_head + off * HD, p.box * HD, &bars->full[s]);
-          bulk_load(sc + b * p.box, p.c.ks + pg * p.c.ks_page + kvh * p.c.ks_head + off, p.box, &bars->full[s]);
-          bulk_load(sc + 64 + b * p.box, p.c.vs + pg * p.c.vs_page + kvh * p.c.vs_head + off, p.box, &bars->full[s]);
-        }
-        if (++s == kRing) { s = 0; ph ^= 1; }
       }
+      pdl_trigger();
     } else if (warp == 1 && lane == 0) {
       // ---------------------------------------------------------------- MMA issuer
       const uint32_t idesc_s = umma_idesc(128, 64, 0, 0), idesc_pv = umma_idesc(128, HD, 0, 0) | (1u << 16);    // V is MN-major
-      const int last = two ? 1 : 0;
       bool ok = true;
-      auto scores = [&](int t) {
-        const int b = t & 1;
-        ok = ok && mbar_wait(&bars->k_full[b], (t >> 1) & 1, abort_word, p.a.err, 752);
-        if (!ok) return;
-        tc_fence_after();
-        for (int q = 0; q <= last; ++q) {
-#pragma unroll
-          for (int k = 0; k < NC * 4; ++k) {
-            const uint64_t da = umma_desc_sw128(sQ + q * Sh::kQTile + (k >> 2) * 16384) + static_cast<uint64_t>((k & 3) * 2);
-            const uint64_t db = umma_desc_sw128(sK + b * Sh::kTile16 + (k >> 2) * 8192) + static_cast<uint64_t>((k & 3) * 2);
-            umma_bf16(tmem_base + q * 128 + b * 64, da, db, idesc_s, k > 0 ? 1u : 0u);
-          }
-          tc_commit(&bars->s_full[q][b]);
-        }
-        tc_commit(&bars->k_empty[b]);
-      };
-      if (nt > 0) scores(0);
-      for (int t = 0; t < nt && ok; ++t) {
-        const int b = t & 1;
-        if (t + 1 < nt) scores(t + 1);              // the product that read P of that buffer was issued before
-        ok = ok && mbar_wait(&bars->v_full[b], (t >> 1) & 1, abort_word, p.a.err, 753);
-        for (int q = 0; q <= last && ok; ++q) {
-          ok = mbar_wait(&bars->p_full[q][b], (t >> 1) & 1, abort_word, p.a.err, 754);
-          if (!ok) break;
+      int ct = 0, cg[2] = {0, 0}, pieces[2] = {0, 0}, done[2] = {0, 0};       // tiles so far: all, and of each query tile; pieces of each; those with tiles
+      for (int i = 0; ok; ++i) {
+        ok = mbar_wait(&bars->piece_full[i % kPieces], (i / kPieces) & 1, abort_word, p.a.err, 766);
+        if (!ok) break;
+        const Piece& pq = bars->piece[i % kPieces];
+        const int nt = pq.nt < 0 ? -1 : pq.tb - pq.ta, last = pq.two;
+        mbar_arrive(&bars->piece_empty[i % kPieces]);
+        if (nt < 0) break;
+        for (int q = 0; q <= last; ++q) ok = ok && mbar_wait(&bars->q_full[q], pieces[q] & 1, abort_word, p.a.err, 762);
+        // S of tile t into the next buffer of each query tile
+        auto scores = [&](int t) {
+          const int b = (ct + t) & 1;
+          ok = ok && mbar_wait(&bars->k_full[b], ((ct + t) >> 1) & 1, abort_word, p.a.err, 752);
+          if (!ok) return;
           tc_fence_after();
+          for (int q = 0; q <= last; ++q) {
+            const int sb = (cg[q] + t) & 1;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tmem_base + 256 + q * 128, tmem_base + q * 128 + b * 64 + k * 8, umma_desc_mn_sw128(sV + b * Sh::kTile16 + k * 2048, 8192, 1024),
-                        idesc_pv, (t > 0 || k > 0) ? 1u : 0u);
-          tc_commit(&bars->pv_done[q][b]);
-          if (q == last) tc_commit(&bars->v_empty[b]);
-          if (t + 1 == nt) tc_commit(&bars->o_done[q]);
+            for (int k = 0; k < NC * 4; ++k) {
+              const uint64_t da = umma_desc_sw128(sQ + q * Sh::kQTile + (k >> 2) * 16384) + static_cast<uint64_t>((k & 3) * 2);
+              const uint64_t db = umma_desc_sw128(sK + b * Sh::kTile16 + (k >> 2) * 8192) + static_cast<uint64_t>((k & 3) * 2);
+              umma_bf16(tmem_base + q * 128 + sb * 64, da, db, idesc_s, k > 0 ? 1u : 0u);
+            }
+            tc_commit(&bars->s_full[q][sb]);
+          }
+          tc_commit(&bars->k_empty[b]);
+        };
+        if (ok && nt > 0) scores(0);
+        for (int t = 0; t < nt && ok; ++t) {
+          const int b = (ct + t) & 1;
+          if (t + 1 < nt) scores(t + 1);            // the product that read P of that buffer was issued before
+          ok = ok && mbar_wait(&bars->v_full[b], ((ct + t) >> 1) & 1, abort_word, p.a.err, 753);
+          for (int q = 0; q <= last && ok; ++q) {
+            const int sb = (cg[q] + t) & 1;
+            if (t == 0) ok = mbar_wait(&bars->o_free[q], (done[q] & 1) ^ 1, abort_word, p.a.err, 763);
+            ok = ok && mbar_wait(&bars->p_full[q][sb], ((cg[q] + t) >> 1) & 1, abort_word, p.a.err, 754);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16_ts(tmem_base + 256 + q * 128, tmem_base + q * 128 + sb * 64 + k * 8, umma_desc_mn_sw128(sV + b * Sh::kTile16 + k * 2048, 8192, 1024),
+                          idesc_pv, (t > 0 || k > 0) ? 1u : 0u);
+            tc_commit(&bars->pv_done[q][sb]);
+            if (q == last) tc_commit(&bars->v_empty[b]);
+            if (t + 1 == nt) tc_commit(&bars->o_done[q]);
+          }
         }
+        ct += nt;
+        for (int q = 0; q <= last; ++q) { cg[q] += nt; ++pieces[q]; done[q] += nt > 0; }
       }
     }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------------------------------------------ codes to f16
-    const int cw = warp - 12, lo = lane & 3, up = (lane >> 2) & 1, quarter = lane >> 3;
-    int s = 0;
+    const int cw = warp - 12;
+    // 16 rows a warp. A quarter-warp reads 128 bytes together; lanes of the row's second half (HD 128) write their two pieces in the other
+    // order, so that the eight meet no bank twice
+    const int chunk = NC == 2 ? (lane & 7) : (lane & 3), row0 = cw * 16 + (NC == 2 ? lane >> 3 : lane >> 2);
+    constexpr int kSteps = NC * 2, kRowStep = 16 / kSteps;
+    const int swap = NC == 2 ? (chunk >> 2) : 0;
+    int s = 0, ct = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int t = 0; t < nt && ok; ++t) {
-      const int b = t & 1, n = min(64, w.kv_hi - (t0 + t) * 64);       // rows behind the last key become zeros
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars->full[s], ph, abort_word, p.a.err, 755))) break;
-      const uint8_t* sc = sScale + s * 128;
-      int top[2];
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint32_t two_bytes = *reinterpret_cast<const uint16_t*>(sc + kv * 64 + 2 * lane);
-        const uint32_t x = 2 * lane < n ? two_bytes & 255u : 0u, y = 2 * lane + 1 < n ? two_bytes >> 8 : 0u;
-        top[kv] = static_cast<int>(__reduce_max_sync(0xffffffffu, max(x, y)));
-      }
-      top[1] = min(max(top[1], kLeastByte), kMostByte);
-      if (warp == 12 && lane == 0) {
-        bars->info[t & 3].k = score_factor(p.a.scale * kLog2e, top[0] - 127 - kHeadroom - qe);
-        bars->info[t & 3].v = static_cast<float>(top[1] - 127);
-        mbar_arrive(&bars->info_full[t & 3]);
-      }
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        ok = __all_sync(0xffffffffu, mbar_wait(kv == 0 ? &bars->k_empty[b] : &bars->v_empty[b], ((t >> 1) & 1) ^ 1, abort_word, p.a.err, 756));
-        if (!ok) break;
-        const uint8_t* from = sRing + s * Sh::kStage + kv * Sh::kCodes;
-        uint8_t* to = (kv == 0 ? sK : sV) + b * Sh::kTile16;
-        // 16 rows a warp. A quarter-warp reads 128 bytes together; lanes of the row's second half (HD 128) write their two pieces in the other
-        // order, so that the eight meet no bank twice
-#pragma unroll
-        for (int it = 0; it < NC * 2; ++it) {
-          const int row = cw * 16 + (NC == 2 ? it * 4 + quarter : it * 8 + quarter * 2 + up), chunk = NC == 2 ? (lane & 7) : lo;
-          uint4 c = *reinterpret_cast<const uint4*>(from + row * HD + chunk * 16);
-          uint32_t f = pow2_f16x2(static_cast<int>(sc[kv * 64 + row]) - top[kv] + kHeadroom);
-          if (row >= n) { c = make_uint4(0, 0, 0, 0); f = 0; }
-          const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
-          const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-          uint32_t h[8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t x[2];
-            codes_f16(words[k], x[0], x[1]);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), f2);
-              h[2 * k + e] = *reinterpret_cast<const uint32_t*>(&y);
-            }
-          }
-          uint8_t* dst = to + (chunk >> 2) * 8192 + row * 128;
-          const int piece = 2 * (chunk & 3), swap = NC == 2 ? (chunk >> 2) : 0;
-          const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), z = make_uint4(h[4], h[5], h[6], h[7]);
-          *reinterpret_cast<uint4*>(dst + (((piece + swap) ^ (row & 7)) << 4)) = swap ? z : a;
-          *reinterpret_cast<uint4*>(dst + (((piece + 1 - swap) ^ (row & 7)) << 4)) = swap ? a : z;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(kv == 0 ? &bars->k_full[b] : &bars->v_full[b]);
-      }
+    for (int i = 0; ok; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->piece_full[i % kPieces], (i / kPieces) & 1, abort_word, p.a.err, 767));
       if (!ok) break;
-      if (lane == 0) mbar_arrive(&bars->empty[s]);
-      if (++s == kRing) { s = 0; ph ^= 1; }
+      const Piece& q = bars->piece[i % kPieces];
+      const int nt = q.nt < 0 ? -1 : q.tb - q.ta;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->piece_empty[i % kPieces]);
+      if (nt < 0) break;
+      for (int t = 0; t < nt && ok; ++t, ++ct) {
+        const int b = ct & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[s], ph, abort_word, p.a.err, 755));
+        if (!ok) break;
+        const int n = bars->rows[s];                 // rows behind the last key become zeros
+        const uint8_t* sc = sScale + s * 128;
+        const uint8_t* from = sRing + s * Sh::kStage + row0 * HD + chunk * 16;
+        // all loads first: the stores that follow could not be told from them
+        uint4 code[2][kSteps];
+        int byte[2][kSteps], top[2];
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t two_bytes = *reinterpret_cast<const uint16_t*>(sc + kv * 64 + 2 * lane);
+          top[kv] = static_cast<int>(max(2 * lane < n ? two_bytes & 255u : 0u, 2 * lane + 1 < n ? two_bytes >> 8 : 0u));
+        }
+#pragma unroll
+        for (int it = 0; it < kSteps; ++it) {
+          code[0][it] = *reinterpret_cast<const uint4*>(from + it * kRowStep * HD);
+          byte[0][it] = sc[row0 + it * kRowStep];
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) top[kv] = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(top[kv])));
+        top[1] = min(max(top[1], kLeastByte), kMostByte);
+        if (warp == 12 && lane == 0) {
+          bars->info[ct & 3].k = top[0] - 127 - kHeadroom;
+          bars->info[ct & 3].v = static_cast<float>(top[1] - 127);
+          mbar_arrive(&bars->info_full[ct & 3]);
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (kv == 1) {
+#pragma unroll
+            for (int it = 0; it < kSteps; ++it) {
+              code[1][it] = *reinterpret_cast<const uint4*>(from + Sh::kCodes + it * kRowStep * HD);
+              byte[1][it] = sc[64 + row0 + it * kRowStep];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->empty[s]);       // all of the stage is in registers
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait(kv == 0 ? &bars->k_empty[b] : &bars->v_empty[b], ((ct >> 1) & 1) ^ 1, abort_word, p.a.err, 756));
+          if (!ok) break;
+          uint8_t* to = (kv == 0 ? sK : sV) + b * Sh::kTile16 + (chunk >> 2) * 8192;
+#pragma unroll
+          for (int it = 0; it < kSteps; ++it) {
+            const int row = row0 + it * kRowStep;
+            uint4 c = code[kv][it];
+            uint32_t f = pow2_f16x2(byte[kv][it] - top[kv] + kHeadroom);
+            if (row >= n) { c = make_uint4(0, 0, 0, 0); f = 0; }
+            const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
+            const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+            uint32_t h[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t x[2];
+              codes_f16(words[k], x[0], x[1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), f2);
+                h[2 * k + e] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+            uint8_t* dst = to + row * 128;
+            const int piece = 2 * (chunk & 3);
+            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+            *reinterpret_cast<uint4*>(dst + (((piece + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
+            *reinterpret_cast<uint4*>(dst + (((piece + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kv == 0 ? &bars->k_full[b] : &bars->v_full[b]);
+        }
+        if (++s == kRing) { s = 0; ph ^= 1; }
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ------------------------------------------------------------------ softmax
-    const int quad = warp & 3;
-    const int limit = valid ? w.kl - w.ql + tq : 0x7fffffff;       // (queries that are not there are zeros: nothing to mask)
-    const bool idle = quad * 32 >= half_tok * G || w.tq0 + g * half_tok + quad * 32 / G >= w.ql;      // no row of this warp is in use
+    const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t s_tile = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + g * 128, o_addr = s_tile + 256;
-    float m = 0.f, l = 0.f;                          // weights and l are relative to m, a lagging running maximum
-    bool ok = true, unset = true;                    // unset: no key has been visible to the row yet
-    const int mine = g == 0 || two ? nt : 0;
-    for (int t = 0; t < mine; ++t) {
-      const int b = t & 1;
-      const uint32_t s_addr = s_tile + b * 64;
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[g][b], (t >> 1) & 1, abort_word, p.a.err, 757));
-      if (!ok) break;
-      if (!idle) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->info_full[t & 3], (t >> 2) & 1, abort_word, p.a.err, 758));
-        if (!ok) break;
-        const float kf = bars->info[t & 3].k, ev = bars->info[t & 3].v;
-        tc_fence_after();
-        uint32_t sr[2][32];
-        tmem_ld_32x32(s_addr, sr[0]);
-        tmem_ld_32x32(s_addr + 32, sr[1]);
-        tc_wait_ld();
-        const int kv0 = (t0 + t) * 64;
-        if (kv0 + 63 > limit) {
+    bool ok = true;
+    int ct = 0, cg = 0, done = 0;                    // tiles so far: all, and of this query tile; its pieces that had tiles
+    int at = 0, qe = 0;                              // the piece whose queries are in place, and their exponent
+    // this thread's query row of the piece, in f16 with the 128-byte swizzle, the largest value in [2^14, 2^15)
+    auto bring_queries = [&]() {
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->piece_full[at % kPieces], (at / kPieces) & 1, abort_word, p.a.err, 768));
+      if (!ok) return;
+      const Piece& w = bars->piece[at % kPieces];
+      if (w.nt < 0 || (g == 1 && !w.two)) return;
+      const int tq = w.tq0 + g * w.half_tok + r / G;
+      const bool valid = r < w.half_tok * G && tq < w.ql && w.qs + tq < p.a.T;
+      const T* src = static_cast<const T*>(p.a.q) + static_cast<int64_t>(valid ? w.qs + tq : 0) * p.a.ldq + static_cast<int64_t>(w.head * G + r % G) * HD;
+      uint4 raw[HD / 8];
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (kv0 + c > limit) sr[c >> 5][c & 31] = __float_as_uint(-INFINITY);
-        }
-        float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      for (int c = 0; c < HD / 8; ++c) raw[c] = valid ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
+      float big = 0.f;
 #pragma unroll
-        for (int c = 0; c < 64; ++c) mxa[c & 3] = fmaxf(mxa[c & 3], __uint_as_float(sr[c >> 5][c & 31]));
-        const float mx = fmaf(fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])), kf, ev);       // kf > 0
-        bool grow = false;
-        if (unset) {
-          unset = mx == -INFINITY;
-          m = unset ? 0.f : mx;
-        } else {
-          grow = mx - m > 8.0f;
-        }
-        if (__any_sync(0xffffffffu, grow)) {
-          ok = t == 0 || mbar_wait(&bars->pv_done[g][(t - 1) & 1], ((t - 1) >> 1) & 1, abort_word, p.a.err, 760);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          const float factor = grow ? exp2f(m - mx) : 1.0f;
-          if (grow) { m = mx; l *= factor; }
+      for (int c = 0; c < HD / 8; ++c) {
+        float x[8];
+        widen8<T>(raw[c], x);
 #pragma unroll
-          for (int q4 = 0; q4 < HD / 32; ++q4) {
-            uint32_t tr[32];
-            tmem_ld_32x32(o_addr + q4 * 32, tr);
-            tc_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 32; ++c) tr[c] = __float_as_uint(__uint_as_float(tr[c]) * factor);
-            tmem_st_32x32(o_addr + q4 * 32, tr);
-          }
-        }
-        float la[4] = {0.f, 0.f, 0.f, 0.f};
-        const float shift = ev - m + kShift;
-        uint32_t pk[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float p0 = ex2(fmaf(__uint_as_float(sr[j >> 4][2 * (j & 15)]), kf, shift));
-          const float p1 = ex2(fmaf(__uint_as_float(sr[j >> 4][2 * (j & 15) + 1]), kf, shift));
-          la[j & 3] += p0 + p1;
-          pk[j] = pack_f16(p0, p1);
-        }
-        tmem_st_32x32(s_addr, pk);
-        l = fmaf((la[0] + la[1]) + (la[2] + la[3]), pow2f(-static_cast<int>(ev)), l);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
+        for (int k = 0; k < 8; ++k) big = fmaxf(big, finite_abs(x[k]));
       }
-      if (lane == 0) mbar_arrive(&bars->p_full[g][b]);
-    }
-    if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[g], 0, abort_word, p.a.err, 761));
-    if (ok && (g == 0 || two)) {
-      tc_fence_after();
-      const float back = 1.f / (1 << kHeadroom);
-      const int64_t out_row = valid ? w.qs + tq : 0;
-      const float f = p.splits > 1 ? back : (l == 0.f ? 0.f : back / l);
-      T* orow = static_cast<T*>(p.a.out) + out_row * p.a.ldo + static_cast<int64_t>(head) * HD;
-      float* part = p.ws + ((static_cast<int64_t>(blockIdx.z) * p.a.T + out_row) * p.a.n_q + head) * (HD + 4);
+      qe = f16_shift(big);
+      const float mul = pow2f(qe);
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        float x[8];
+        widen8<T>(raw[c], x);
+        uint8_t* row = sQ + g * Sh::kQTile + (c >> 3) * 16384 + r * 128;
+        *reinterpret_cast<uint4*>(row + (((c & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pack_f16(x[0] * mul, x[1] * mul), pack_f16(x[2] * mul, x[3] * mul), pack_f16(x[4] * mul, x[5] * mul), pack_f16(x[6] * mul, x[7] * mul));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full[g]);
+    };
+    bring_queries();
+    while (ok) {
+      const Piece& cur = bars->piece[at % kPieces];
+      const int nt = cur.tb - cur.ta, ta = cur.ta, my_qe = qe, tq = cur.tq0 + g * cur.half_tok + r / G;
+      if (cur.nt < 0) break;
+      const bool active = g == 0 || cur.two, my_row = active && r < cur.half_tok * G && tq < cur.ql && cur.qs + tq < p.a.T;
+      const int limit = my_row ? cur.kl - cur.ql + tq : 0x7fffffff;          // (queries that are not there are zeros: nothing to mask)
+      const bool idle = __all_sync(0xffffffffu, !my_row);                    // no row of this warp is in use
+      float m = 0.f, l = 0.f;                        // weights and l are relative to m, a lagging running maximum
+      bool unset = true;                             // no key has been visible to the row yet
+      for (int t = 0; t < nt && active && ok; ++t) {
+        const int b = (cg + t) & 1;
+        const uint32_t s_addr = s_tile + b * 64;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[g][b], ((cg + t) >> 1) & 1, abort_word, p.a.err, 757));
+        if (!ok) break;
+        if (!idle) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->info_full[(ct + t) & 3], ((ct + t) >> 2) & 1, abort_word, p.a.err, 758));
+          if (!ok) break;
+          const float kf = score_factor(p.a.scale * kLog2e, bars->info[(ct + t) & 3].k - my_qe), ev = bars->info[(ct + t) & 3].v;
+          tc_fence_after();
+          uint32_t sr[2][32];
+          tmem_ld_32x32(s_addr, sr[0]);
+          tmem_ld_32x32(s_addr + 32, sr[1]);
+          tc_wait_ld();
+          const int kv0 = (ta + t) * 64;
+          if (kv0 + 63 > limit) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (kv0 + c > limit) sr[c >> 5][c & 31] = __float_as_uint(-INFINITY);
+          }
+          float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 64; ++c) mxa[c & 3] = fmaxf(mxa[c & 3], __uint_as_float(sr[c >> 5][c & 31]));
+          const float mx = fmaf(fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])), kf, ev);       // kf > 0
+          bool grow = false;
+          if (unset) {
+            unset = mx == -INFINITY;
+            m = unset ? 0.f : mx;
+          } else {
+            grow = mx - m > 8.0f;
+          }
+          if (__any_sync(0xffffffffu, grow)) {
+            // the last P . V may still be adding
+            ok = t == 0 || mbar_wait(&bars->pv_done[g][b ^ 1], ((cg + t - 1) >> 1) & 1, abort_word, p.a.err, 760);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const float factor = grow ? exp2f(m - mx) : 1.0f;
+            if (grow) { m = mx; l *= factor; }
+#pragma unroll
+            for (int q4 = 0; q4 < HD / 32; ++q4) {
+              uint32_t tr[32];
+              tmem_ld_32x32(o_addr + q4 * 32, tr);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) tr[c] = __float_as_uint(__uint_as_float(tr[c]) * factor);
+              tmem_st_32x32(o_addr + q4 * 32, tr);
+            }
+          }
+          float la[4] = {0.f, 0.f, 0.f, 0.f};
+          const float shift = ev - m + kShift;
+          uint32_t pk[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float p0 = ex2(fmaf(__uint_as_float(sr[j >> 4][2 * (j & 15)]), kf, shift));
+            const float p1 = ex2(fmaf(__uint_as_float(sr[j >> 4][2 * (j & 15) + 1]), kf, shift));
+            la[j & 3] += p0 + p1;
+            pk[j] = pack_f16(p0, p1);
+          }
+          tmem_st_32x32(s_addr, pk);
+          l = fmaf((la[0] + la[1]) + (la[2] + la[3]), pow2f(-static_cast<int>(ev)), l);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&bars->p_full[g][b]);
+      }
+      // all scores of this piece have been made: its queries may go
+      ct += nt;
+      if (active) cg += nt;
+      if (!ok) break;
+      const bool whole = ta == 0 && nt == cur.nt;
+      const int row = cur.qs + tq, head = cur.head * G + r % G;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->piece_empty[at % kPieces]);
+      ++at;
+      bring_queries();
+      if (!ok) break;
+      if (!active) continue;
+      if (nt > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[g], done & 1, abort_word, p.a.err, 761));
+        if (!ok) break;
+        ++done;
+        tc_fence_after();
+      }
+      const float f = (whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f) * (1.f / (1 << kHeadroom));
+      T* orow = static_cast<T*>(p.a.out) + static_cast<int64_t>(my_row ? row : 0) * p.a.ldo + static_cast<int64_t>(head) * HD;
+      // a piece that begins its CTA's share goes to slot 0, one that ends it to slot 1
+      float* part = p.ws + ((static_cast<int64_t>(cta) * 2 + (ta > 0 ? 0 : 1)) * 256 + g * 128 + r) * (HD + 4);
 #pragma unroll
       for (int q4 = 0; q4 < HD / 32; ++q4) {
-        uint32_t ta[32];
-        if (mine > 0) {
-          tmem_ld_32x32(o_addr + q4 * 32, ta);      // warp-collective
+        uint32_t tr[32];
+        if (nt > 0) {
+          tmem_ld_32x32(o_addr + q4 * 32, tr);      // warp-collective
           tc_wait_ld();
         } else {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) ta[c] = 0;
+          for (int c = 0; c < 32; ++c) tr[c] = 0;
         }
-        if (valid) {
+        if (my_row) {
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
-            const float4 v = make_float4(__uint_as_float(ta[c]), __uint_as_float(ta[c + 1]), __uint_as_float(ta[c + 2]), __uint_as_float(ta[c + 3]));
-            if (p.splits == 1) store4(orow + q4 * 32 + c, v, f);
+            const float4 v = make_float4(__uint_as_float(tr[c]), __uint_as_float(tr[c + 1]), __uint_as_float(tr[c + 2]), __uint_as_float(tr[c + 3]));
+            if (whole) store4(orow + q4 * 32 + c, v, f);
             else *reinterpret_cast<float4*>(part + q4 * 32 + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
           }
         }
       }
-      if (valid && p.splits > 1) { part[HD] = unset ? kNoMax : m; part[HD + 1] = l; }
+      if (my_row && !whole) { part[HD] = unset ? kNoMax : m; part[HD + 1] = l; }
+      if (nt > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->o_free[g]);
+      }
     }
   }
 
@@ -451,51 +633,63 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   }
 }
 
-// The parts of each row, added up: a block per (plan tile, head), a warp per row in turn.
+// Segments that lie in several shares. A block (times four, for 64 rows each) per border between two shares; the first border inside a segment adds its
+// pieces up, a warp per row in turn.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(256) join_chunks_kernel(const __grid_constant__ ChunkParams p, int ctas) {
   pdl_wait();
   const MbFp8Attention& a = p.a;
-  const int G = a.n_q / a.n_kv, tok = 64 / G, tile = blockIdx.y, kvh = blockIdx.x;
-  const int seq = a.tile_seq[tile];
-  if (seq < 0) return;
-  const int tq0 = a.tile_q0[tile], ql = a.q_len[seq], qs = a.q_start[seq];
-  const int rows = (min(tq0 + tok, ql) - tq0) * G, lane = threadIdx.x & 31;
+  const int n = a.n_tiles, per_head = p.sums[n], G = a.n_q / a.n_kv, border = blockIdx.x + 1;
+  const int64_t U = static_cast<int64_t>(per_head) * a.n_kv;
+  const int C = chunk_shares(U, ctas);
+  if (border >= C || U == 0) return;
+  const int64_t u = chunk_start(U, C, border);
+  const int head = static_cast<int>(u / per_head), v = static_cast<int>(u - static_cast<int64_t>(head) * per_head);
+  const int tile = tile_holding(p.sums, n, v);
+  const int len = p.sums[tile + 1] - p.sums[tile], nt = len - kSetup;
+  if (v - p.sums[tile] <= kSetup || nt <= 0) return;          // no tile of the segment lies before the border
+  const int64_t first = static_cast<int64_t>(head) * per_head + p.sums[tile] + kSetup;
+  const int c0 = chunk_holding(U, C, first), c1 = chunk_holding(U, C, first + nt - 1);
+  if (c0 != border - 1 || c0 == c1) return;                   // an earlier border's work
+  Work w;
+  if (!work_of(a, tile, w)) return;
+  const int lane = threadIdx.x & 31;
   constexpr int PER = HD / 32;
-  for (int r = threadIdx.x >> 5; r < rows; r += 8) {
-    const int64_t row = qs + tq0 + r / G;
-    if (row >= a.T) continue;
-    const int head = kvh * G + r % G;
-    const float* part = p.ws + (row * a.n_q + head) * (HD + 4);
-    const int64_t step = static_cast<int64_t>(a.T) * a.n_q * (HD + 4);
+  constexpr int64_t kSlot = 256 * (HD + 4);
+  for (int i = threadIdx.x >> 5; i < 64; i += 8) {
+    const int at = blockIdx.y * 64 + i, g = at >> 7, r = at & 127;
+    const int tq = w.tq0 + g * w.half_tok + r / G;
+    if (r >= w.half_tok * G || tq >= w.ql || w.qs + tq >= a.T) continue;
+    // the first piece ends its share (slot 1), the others begin theirs (slot 0)
+    const float* row = p.ws + static_cast<int64_t>(c0) * 2 * kSlot + at * (HD + 4);
+    auto piece = [&](int k) { return row + (2 * k + (k == 0 ? 1 : 0)) * kSlot; };
+    const int pieces = c1 - c0 + 1;
     float m = kNoMax;
-    for (int z = 0; z < p.splits; ++z) m = fmaxf(m, part[z * step + HD]);
+    for (int k = lane; k < pieces; k += 32) m = fmaxf(m, piece(k)[HD]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float l = 0.f, o[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = 0.f;
-    for (int z = 0; z < p.splits; ++z) {
-      const float* q = part + z * step;
+    for (int c = 0; c < PER; ++c) o[c] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k) {
+      const float* q = piece(k);
       const float f = exp2f(q[HD] - m);
       l = fmaf(q[HD + 1], f, l);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] = fmaf(q[lane * PER + i], f, o[i]);
+      for (int c = 0; c < PER; ++c) o[c] = fmaf(q[lane * PER + c], f, o[c]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* dst = static_cast<T*>(a.out) + row * a.ldo + static_cast<int64_t>(head) * HD + lane * PER;
+    T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(w.qs + tq) * a.ldo + static_cast<int64_t>(head * G + r % G) * HD + lane * PER;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) dst[i] = static_cast<T>(o[i] * inv);
+    for (int c = 0; c < PER; ++c) dst[c] = static_cast<T>(o[c] * inv);
   }
 }
 
-// Parts per CTA's keys: as many as give every SM a CTA. A sequence of the plan has one CTA per head at least, four plan tiles at most share one.
-static int chunk_splits(const MbFp8Attention& a, int num_sms) {
-  const int ctas = max((a.n_tiles + 3) / 4, min(a.n_tiles, a.B - a.n_decode)) * a.n_kv;
-  return max(1, min(kMaxSplits, num_sms / max(1, ctas)));
-}
+static size_t slots_bytes(const MbFp8Attention& a, int num_sms) { return static_cast<size_t>(num_sms) * 2 * 256 * (a.head_dim + 4) * sizeof(float); }
 
 size_t chunk_workspace(const MbFp8Attention& a, int num_sms) {
-  const int s = a.n_tiles > 0 ? chunk_splits(a, num_sms) : 1;
-  return s > 1 ? static_cast<size_t>(s) * a.T * a.n_q * (a.head_dim + 4) * sizeof(float) : 0;
+  return a.n_tiles > 0 ? slots_bytes(a, num_sms) + (min(a.n_tiles, kMaxTiles) + 1) * sizeof(int) : 0;
 }
 
 template <int HD, typename T>
@@ -506,23 +700,29 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
     // the register split inside the kernel adds up to what 512 threads of 128 registers bring along
     cudaFuncAttributes at;
     if (cudaFuncGetAttributes(&at, kern) != cudaSuccess || at.numRegs != 128) return MB_ERR_LAUNCH;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<HD>::kSmem)) != cudaSuccess) return MB_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<HD>::kSmem + (kMaxTiles + 1) * sizeof(int))) != cudaSuccess)
+      return MB_ERR_LAUNCH;
     configured.done();
   }
   ChunkParams p = {};
-  p.a = a;
   p.c = c;
   p.ws = static_cast<float*>(a.ws);
-  p.splits = chunk_splits(a, num_sms);
+  p.sums = reinterpret_cast<int*>(static_cast<char*>(a.ws) + slots_bytes(a, num_sms));
   p.box = c.page_size % 64 == 0 ? 64 : c.page_size % 32 == 0 ? 32 : 16;
-  if (launch_k(kern, dim3(a.n_kv, a.n_tiles, p.splits), dim3(kThreads), Shape<HD>::kSmem, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
-  if (p.splits > 1 && launch_k(chunk_join_kernel<HD, T>, dim3(a.n_kv, a.n_tiles), dim3(256), 0, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
+  for (int at = 0; at < a.n_tiles; at += kMaxTiles) {
+    p.a = a;
+    p.a.tile_seq = a.tile_seq + at;
+    p.a.tile_q0 = a.tile_q0 + at;
+    p.a.n_tiles = min(kMaxTiles, a.n_tiles - at);
+    const size_t smem = Shape<HD>::kSmem + (p.a.n_tiles + 1) * sizeof(int);
+    if (launch_k(kern, dim3(num_sms), dim3(kThreads), smem, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
+    if (num_sms > 1 && launch_k(join_chunks_kernel<HD, T>, dim3(num_sms - 1, 4), dim3(256), 0, stream, p, num_sms) != cudaSuccess) return MB_ERR_LAUNCH;
+  }
   return MB_OK;
 }
 
 int chunk_attention(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cudaStream_t stream) {
   if (a.n_tiles <= 0) return MB_OK;
-  if (a.n_tiles > 65535) return MB_ERR_TOO_LARGE;
   if (a.ws_bytes < chunk_workspace(a, num_sms)) return MB_ERR_TOO_LARGE;
   if (a.head_dim == 128) return a.dtype == 0 ? launch<128, __nv_bfloat16>(a, c, num_sms, stream) : launch<128, __half>(a, c, num_sms, stream);
   return a.dtype == 0 ? launch<64, __nv_bfloat16>(a, c, num_sms, stream) : launch<64, __half>(a, c, num_sms, stream);
