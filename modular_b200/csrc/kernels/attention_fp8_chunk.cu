@@ -230,9 +230,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   const int64_t U = static_cast<int64_t>(run) * p.a.n_kv;
   const int C = chunk_shares(U, gridDim.x), cta = blockIdx.x;
 
-  // 512 x 128 registers at launch = 128 x (48 + 192 + 192 + 80)
+  // 512 x 128 registers at launch = 128 x (88 + 160 + 160 + 104)
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 2 && lane == 0) {
       // ---------------------------------------------------------------- pieces
       Pieces pc;
@@ -307,63 +307,95 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         }
       }
       pdl_trigger();
-    } else if (warp == 1 && lane == 0) {
-      // ---------------------------------------------------------------- MMA issuer
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer: the warp as a whole keeps count, so that descriptors and addresses
+      // are the same for all lanes and lie in uniform registers; one lane issues. (With one lane alone an instruction took 110 cycles to issue.)
       const uint32_t idesc_s = umma_idesc(128, 64, 0, 0), idesc_pv = umma_idesc(128, HD, 0, 0) | (1u << 16);    // V is MN-major
+      const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, 8192, 1024);
       bool ok = true;
-      int ct = 0, cg[2] = {0, 0}, pieces[2] = {0, 0}, done[2] = {0, 0};       // tiles so far: all, and of each query tile; pieces of each; those with tiles
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_word, p.a.err, code)); };
+      // parities, each flipped where a wait on it has been passed: buffers of K and V, score buffers, pieces of a query tile
+      uint32_t kb = 0, k_ph = 0, vb = 0, v_ph = 0;            // buffer, and its phase
+      uint32_t sb0 = 0, sb1 = 0, pb0 = 0, pb1 = 0, p_ph0 = 0, p_ph1 = 0;     // next score buffer; buffer of the next weights, and its phase
+      uint32_t q_ph0 = 0, q_ph1 = 0, o_ph0 = 1, o_ph1 = 1;
+      // S of the next keys into the next buffer of each query tile
+      auto scores_of = [&](uint64_t qd, uint64_t kd, uint32_t tmem, uint64_t* full) {
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < NC * 4; ++k)
+            umma_bf16(tmem, qd + static_cast<uint64_t>((k >> 2) * (16384 >> 4) + (k & 3) * 2), kd + static_cast<uint64_t>((k >> 2) * (8192 >> 4) + (k & 3) * 2), idesc_s,
+                      k > 0 ? 1u : 0u);
+          tc_commit(full);
+        }
+        __syncwarp();
+      };
+      auto scores = [&](bool two) {
+        wait(&bars->k_full[kb], k_ph, 752);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t kd = k_desc + static_cast<uint64_t>(kb * (Sh::kTile16 >> 4));
+        scores_of(q_desc, kd, tmem_base + sb0 * 64, &bars->s_full[0][sb0]);
+        sb0 ^= 1;
+        if (two) {
+          scores_of(q_desc + static_cast<uint64_t>(Sh::kQTile >> 4), kd, tmem_base + 128 + sb1 * 64, &bars->s_full[1][sb1]);
+          sb1 ^= 1;
+        }
+        if (elect_one()) tc_commit(&bars->k_empty[kb]);
+        __syncwarp();
+        kb ^= 1;
+        k_ph ^= kb ^ 1;
+      };
+      auto product = [&](uint64_t vd, uint32_t tmem_o, uint32_t tmem_p, bool first, uint64_t* done, uint64_t* empty, uint64_t* all) {
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ts(tmem_o, tmem_p + k * 8, vd + static_cast<uint64_t>(k * (2048 >> 4)), idesc_pv, (!first || k > 0) ? 1u : 0u);
+          tc_commit(done);
+          if (empty) tc_commit(empty);
+          if (all) tc_commit(all);
+        }
+        __syncwarp();
+      };
       for (int i = 0; ok; ++i) {
-        ok = mbar_wait(&bars->piece_full[i % kPieces], (i / kPieces) & 1, abort_word, p.a.err, 766);
+        wait(&bars->piece_full[i % kPieces], (i / kPieces) & 1, 766);
         if (!ok) break;
         const Piece& pq = bars->piece[i % kPieces];
-        const int nt = pq.nt < 0 ? -1 : pq.tb - pq.ta, last = pq.two;
-        mbar_arrive(&bars->piece_empty[i % kPieces]);
+        const int nt = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(pq.nt < 0 ? 0 : pq.tb - pq.ta + 1))) - 1;
+        const bool two = __all_sync(0xffffffffu, pq.nt >= 0 && pq.two != 0);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->piece_empty[i % kPieces]);
         if (nt < 0) break;
-        for (int q = 0; q <= last; ++q) ok = ok && mbar_wait(&bars->q_full[q], pieces[q] & 1, abort_word, p.a.err, 762);
-        // S of tile t into the next buffer of each query tile
-        auto scores = [&](int t) {
-          const int b = (ct + t) & 1;
-          ok = ok && mbar_wait(&bars->k_full[b], ((ct + t) >> 1) & 1, abort_word, p.a.err, 752);
-          if (!ok) return;
-          tc_fence_after();
-          for (int q = 0; q <= last; ++q) {
-            const int sb = (cg[q] + t) & 1;
-#pragma unroll
-            for (int k = 0; k < NC * 4; ++k) {
-              const uint64_t da = umma_desc_sw128(sQ + q * Sh::kQTile + (k >> 2) * 16384) + static_cast<uint64_t>((k & 3) * 2);
-              const uint64_t db = umma_desc_sw128(sK + b * Sh::kTile16 + (k >> 2) * 8192) + static_cast<uint64_t>((k & 3) * 2);
-              umma_bf16(tmem_base + q * 128 + sb * 64, da, db, idesc_s, k > 0 ? 1u : 0u);
-            }
-            tc_commit(&bars->s_full[q][sb]);
-          }
-          tc_commit(&bars->k_empty[b]);
-        };
-        if (ok && nt > 0) scores(0);
+        wait(&bars->q_full[0], q_ph0, 762);
+        q_ph0 ^= 1;
+        if (two) { wait(&bars->q_full[1], q_ph1, 762); q_ph1 ^= 1; }
+        if (ok && nt > 0) scores(two);
         for (int t = 0; t < nt && ok; ++t) {
-          const int b = (ct + t) & 1;
-          if (t + 1 < nt) scores(t + 1);            // the product that read P of that buffer was issued before
-          ok = ok && mbar_wait(&bars->v_full[b], ((ct + t) >> 1) & 1, abort_word, p.a.err, 753);
-          for (int q = 0; q <= last && ok; ++q) {
-            const int sb = (cg[q] + t) & 1;
-            if (t == 0) ok = mbar_wait(&bars->o_free[q], (done[q] & 1) ^ 1, abort_word, p.a.err, 763);
-            ok = ok && mbar_wait(&bars->p_full[q][sb], ((cg[q] + t) >> 1) & 1, abort_word, p.a.err, 754);
+          if (t + 1 < nt) scores(two);              // the product that read P of that buffer was issued before
+          wait(&bars->v_full[vb], v_ph, 753);
+          const uint64_t vd = v_desc + static_cast<uint64_t>(vb * (Sh::kTile16 >> 4));
+          uint64_t* empty = &bars->v_empty[vb];
+          vb ^= 1;
+          v_ph ^= vb ^ 1;
+          if (t == 0) { wait(&bars->o_free[0], o_ph0, 763); o_ph0 ^= 1; }
+          wait(&bars->p_full[0][pb0], p_ph0, 754);
+          if (!ok) break;
+          product(vd, tmem_base + 256, tmem_base + pb0 * 64, t == 0, &bars->pv_done[0][pb0], two ? nullptr : empty, t + 1 == nt ? &bars->o_done[0] : nullptr);
+          pb0 ^= 1;
+          p_ph0 ^= pb0 ^ 1;
+          if (two) {
+            if (t == 0) { wait(&bars->o_free[1], o_ph1, 763); o_ph1 ^= 1; }
+            wait(&bars->p_full[1][pb1], p_ph1, 754);
             if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16_ts(tmem_base + 256 + q * 128, tmem_base + q * 128 + sb * 64 + k * 8, umma_desc_mn_sw128(sV + b * Sh::kTile16 + k * 2048, 8192, 1024),
-                          idesc_pv, (t > 0 || k > 0) ? 1u : 0u);
-            tc_commit(&bars->pv_done[q][sb]);
-            if (q == last) tc_commit(&bars->v_empty[b]);
-            if (t + 1 == nt) tc_commit(&bars->o_done[q]);
+            product(vd, tmem_base + 384, tmem_base + 128 + pb1 * 64, t == 0, &bars->pv_done[1][pb1], empty, t + 1 == nt ? &bars->o_done[1] : nullptr);
+            pb1 ^= 1;
+            p_ph1 ^= pb1 ^ 1;
           }
         }
-        ct += nt;
-        for (int q = 0; q <= last; ++q) { cg[q] += nt; ++pieces[q]; done[q] += nt > 0; }
       }
     }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     // ------------------------------------------------------------------ codes to f16
     const int cw = warp - 12;
     // 16 rows a warp. A quarter-warp reads 128 bytes together; lanes of the row's second half (HD 128) write their two pieces in the other
@@ -457,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     // ------------------------------------------------------------------ softmax
     const int g = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t s_tile = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + g * 128, o_addr = s_tile + 256;
