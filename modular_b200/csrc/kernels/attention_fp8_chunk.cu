@@ -44,8 +44,7 @@ struct ChunkParams {
 };
 
 struct TileInfo {
-  int k;                                // exponents left over
-  float v;
+  float k, v;                           // factor of a score, exponent of the values
 };
 // Tiles [ta, tb) of a segment's nt, as warp 2 hands them out
 struct Piece {
@@ -103,10 +102,10 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       : "memory");
 }
 
-// 2^x as f16 in both halves, x <= 6; zero below the smallest subnormal
-__device__ __forceinline__ uint32_t pow2_f16x2(int x) {
-  const uint32_t h = x >= -14 ? static_cast<uint32_t>(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u;
-  return h | (h << 16);
+// 2^(byte - top + kHeadroom) as f16 in both halves; below 2^-24 it is zero
+__device__ __forceinline__ uint32_t relative_scale(int byte, int top) {
+  const float f = __uint_as_float(static_cast<uint32_t>(max(byte + (127 + kHeadroom - top), 0)) << 23);
+  return pack_f16(f, f);
 }
 
 // A segment of the plan. Plan tiles hold 64 / G tokens; a segment takes up to four of them, the first at a multiple of four.
@@ -398,11 +397,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     // ------------------------------------------------------------------ codes to f16
     const int cw = warp - 12;
-    // 16 rows a warp. A quarter-warp reads 128 bytes together; lanes of the row's second half (HD 128) write their two pieces in the other
-    // order, so that the eight meet no bank twice
-    const int chunk = NC == 2 ? (lane & 7) : (lane & 3), row0 = cw * 16 + (NC == 2 ? lane >> 3 : lane >> 2);
+    // 16 rows a warp, 16 codes a lane and step. With HD 128 the lanes of a quarter-warp take the first half of one row and the second half of its
+    // neighbour: they read from all banks, and their writes, to the same places of two operand chunks, fall on different banks through the swizzle
+    const int chunk = NC == 2 ? (lane & 7) : (lane & 3), row0 = cw * 16 + (NC == 2 ? (lane >> 3) ^ (chunk >> 2) : lane >> 2);
     constexpr int kSteps = NC * 2, kRowStep = 16 / kSteps;
-    const int swap = NC == 2 ? (chunk >> 2) : 0;
+    const int piece = 2 * (chunk & 3);
+    const uint32_t to_lo = (chunk >> 2) * 8192 + row0 * 128 + ((piece ^ (row0 & 7)) << 4), to_hi = to_lo ^ 16;
     int s = 0, ct = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         const int b = ct & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[s], ph, abort_word, p.a.err, 755));
         if (!ok) break;
-        const int n = bars->rows[s];                 // rows behind the last key become zeros
+        const int n = bars->rows[s];
         const uint8_t* sc = sScale + s * 128;
         const uint8_t* from = sRing + s * Sh::kStage + row0 * HD + chunk * 16;
         // all loads first: the stores that follow could not be told from them
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         for (int kv = 0; kv < 2; ++kv) top[kv] = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(top[kv])));
         top[1] = min(max(top[1], kLeastByte), kMostByte);
         if (warp == 12 && lane == 0) {
-          bars->info[ct & 3].k = top[0] - 127 - kHeadroom;
+          bars->info[ct & 3].k = score_factor(p.a.scale * kLog2e, top[0] - 127 - kHeadroom);
           bars->info[ct & 3].v = static_cast<float>(top[1] - 127);
           mbar_arrive(&bars->info_full[ct & 3]);
         }
@@ -455,14 +455,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           }
           ok = __all_sync(0xffffffffu, mbar_wait(kv == 0 ? &bars->k_empty[b] : &bars->v_empty[b], ((ct >> 1) & 1) ^ 1, abort_word, p.a.err, 756));
           if (!ok) break;
-          uint8_t* to = (kv == 0 ? sK : sV) + b * Sh::kTile16 + (chunk >> 2) * 8192;
+          uint8_t* to = (kv == 0 ? sK : sV) + b * Sh::kTile16;
+          if (n < 64) {                              // rows behind the last key become zeros
+#pragma unroll
+            for (int it = 0; it < kSteps; ++it)
+              if (row0 + it * kRowStep >= n) { code[kv][it] = make_uint4(0, 0, 0, 0); byte[kv][it] = 0; }
+          }
 #pragma unroll
           for (int it = 0; it < kSteps; ++it) {
-            const int row = row0 + it * kRowStep;
-            uint4 c = code[kv][it];
-            uint32_t f = pow2_f16x2(byte[kv][it] - top[kv] + kHeadroom);
-            if (row >= n) { c = make_uint4(0, 0, 0, 0); f = 0; }
+            const uint32_t f = relative_scale(byte[kv][it], top[kv]);
             const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
+            const uint4 c = code[kv][it];
             const uint32_t words[4] = {c.x, c.y, c.z, c.w};
             uint32_t h[8];
 #pragma unroll
@@ -475,11 +478,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 h[2 * k + e] = *reinterpret_cast<const uint32_t*>(&y);
               }
             }
-            uint8_t* dst = to + row * 128;
-            const int piece = 2 * (chunk & 3);
-            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-            *reinterpret_cast<uint4*>(dst + (((piece + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
-            *reinterpret_cast<uint4*>(dst + (((piece + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
+            // (four rows on the swizzle has another bit set: the place moves by 64 bytes the other way)
+            const uint32_t turn = NC == 2 ? (it & 1) << 6 : 0u;
+            *reinterpret_cast<uint4*>(to + ((to_lo ^ turn) + it * kRowStep * 128)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(to + ((to_hi ^ turn) + it * kRowStep * 128)) = make_uint4(h[4], h[5], h[6], h[7]);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -533,7 +535,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     bring_queries();
     while (ok) {
       const Piece& cur = bars->piece[at % kPieces];
-      const int nt = cur.tb - cur.ta, ta = cur.ta, my_qe = qe, tq = cur.tq0 + g * cur.half_tok + r / G;
+      const float my_back = pow2f(-qe);
+      const int nt = cur.tb - cur.ta, ta = cur.ta, tq = cur.tq0 + g * cur.half_tok + r / G;
       if (cur.nt < 0) break;
       const bool active = g == 0 || cur.two, my_row = active && r < cur.half_tok * G && tq < cur.ql && cur.qs + tq < p.a.T;
       const int limit = my_row ? cur.kl - cur.ql + tq : 0x7fffffff;          // (queries that are not there are zeros: nothing to mask)
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         if (!idle) {
           ok = __all_sync(0xffffffffu, mbar_wait(&bars->info_full[(ct + t) & 3], ((ct + t) >> 2) & 1, abort_word, p.a.err, 758));
           if (!ok) break;
-          const float kf = score_factor(p.a.scale * kLog2e, bars->info[(ct + t) & 3].k - my_qe), ev = bars->info[(ct + t) & 3].v;
+          const float kf = fminf(fmaxf(bars->info[(ct + t) & 3].k * my_back, 1.1754944e-38f), 8.5e37f), ev = bars->info[(ct + t) & 3].v;       // (never zero)
           tc_fence_after();
           uint32_t sr[2][32];
           tmem_ld_32x32(s_addr, sr[0]);
@@ -562,8 +565,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           }
           float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 64; ++c) mxa[c & 3] = fmaxf(mxa[c & 3], __uint_as_float(sr[c >> 5][c & 31]));
-          const float mx = fmaf(fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])), kf, ev);       // kf > 0
+          for (int c = 0; c < 64; c += 2) mxa[(c >> 1) & 3] = max3(mxa[(c >> 1) & 3], __uint_as_float(sr[c >> 5][c & 31]), __uint_as_float(sr[c >> 5][(c & 31) + 1]));
+          const float mx = fmaf(fmaxf(max3(mxa[0], mxa[1], mxa[2]), mxa[3]), kf, ev);       // kf > 0
           bool grow = false;
           if (unset) {
             unset = mx == -INFINITY;
@@ -589,18 +592,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
               tmem_st_32x32(o_addr + q4 * 32, tr);
             }
           }
-          float la[4] = {0.f, 0.f, 0.f, 0.f};
+          uint64_t la[2] = {0, 0};
           const float shift = ev - m + kShift;
+          const uint64_t kf2 = two_f32(kf, kf), shift2 = two_f32(shift, shift);
           uint32_t pk[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float p0 = ex2(fmaf(__uint_as_float(sr[j >> 4][2 * (j & 15)]), kf, shift));
-            const float p1 = ex2(fmaf(__uint_as_float(sr[j >> 4][2 * (j & 15) + 1]), kf, shift));
-            la[j & 3] += p0 + p1;
+            float p0, p1;
+            of_two_f32(fma2(two_f32(__uint_as_float(sr[j >> 4][2 * (j & 15)]), __uint_as_float(sr[j >> 4][2 * (j & 15) + 1])), kf2, shift2), p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            la[j & 1] = add2(la[j & 1], two_f32(p0, p1));
             pk[j] = pack_f16(p0, p1);
           }
           tmem_st_32x32(s_addr, pk);
-          l = fmaf((la[0] + la[1]) + (la[2] + la[3]), pow2f(-static_cast<int>(ev)), l);
+          float l0, l1;
+          of_two_f32(add2(la[0], la[1]), l0, l1);
+          l = fmaf(l0 + l1, pow2f(-static_cast<int>(ev)), l);
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
