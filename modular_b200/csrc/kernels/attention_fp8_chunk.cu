@@ -8,7 +8,7 @@
 //   warp 0        producer: codes and exponents of 64 tokens (bulk copies, the rows of a page and head lie together) into a ring
 //   warps 12-15   codes to f16, into operand tiles with the 128-byte swizzle. Within a tile a row's scale is applied relative to the largest
 //                 of the tile (a power of two: exact unless it is 2^-20 of that), so the tile has one scale left over, for K and for V
-//   warp 1        MMA issuer: S_g = Q_g . K^T of the next keys into the other of two buffers, then O_g += P_g . V (P from TMEM)
+//   warps 1, 3    MMA issuers, one per query tile: S_g = Q_g . K^T of the next keys into the other of two buffers, then O_g += P_g . V (P from TMEM)
 //   warps 4-11    softmax, a query row per thread (as attention_tc.cu). The tile's scale of K is part of the score's factor; that of V, 2^E, goes
 //                 into the exponent, 2^(t + E - m), and the denominator adds the tile's sum times 2^-E. The next segment's queries are brought in
 //                 before the results of this one are read
@@ -53,7 +53,7 @@ struct Piece {
   int qs, ql, kl, kv_hi;
 };
 constexpr int kPieces = 4;
-constexpr int kRoles = 14;              // warps that take them: producer, MMA issuer, four converters, eight of softmax
+constexpr int kRoles = 15;              // warps that take them: producer, two MMA issuers, four converters, eight of softmax
 
 struct ChunkBars {
   uint64_t full[kRing], empty[kRing];
@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   if (tid == 0) {
     for (int s = 0; s < kRing; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 4); }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&bars->k_full[b], 4); mbar_init(&bars->k_empty[b], 1);
-      mbar_init(&bars->v_full[b], 4); mbar_init(&bars->v_empty[b], 1);
+      mbar_init(&bars->k_full[b], 4); mbar_init(&bars->k_empty[b], 2);
+      mbar_init(&bars->v_full[b], 4); mbar_init(&bars->v_empty[b], 2);
       for (int g = 0; g < 2; ++g) { mbar_init(&bars->s_full[g][b], 1); mbar_init(&bars->p_full[g][b], 4); mbar_init(&bars->pv_done[g][b], 1); }
       mbar_init(&bars->q_full[b], 4); mbar_init(&bars->o_done[b], 1); mbar_init(&bars->o_free[b], 4);
     }
@@ -306,90 +306,81 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         }
       }
       pdl_trigger();
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer: the warp as a whole keeps count, so that descriptors and addresses
-      // are the same for all lanes and lie in uniform registers; one lane issues. (With one lane alone an instruction took 110 cycles to issue.)
+    } else if (warp == 1 || warp == 3) {
+      // ---------------------------------------------------------------- MMA issuers, a warp per query tile: while one waits, the other's MMAs run. The
+      // warp as a whole keeps count, so that descriptors and addresses are the same for all lanes and lie in uniform registers; one lane issues. (With
+      // one lane alone an instruction took 110 cycles to issue.)
       const uint32_t idesc_s = umma_idesc(128, 64, 0, 0), idesc_pv = umma_idesc(128, HD, 0, 0) | (1u << 16);    // V is MN-major
-      const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, 8192, 1024);
+      const bool second = warp == 3;
+      const uint64_t q_desc = umma_desc_sw128(sQ + (second ? Sh::kQTile : 0)), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, 8192, 1024);
+      const uint32_t tmem_s = tmem_base + (second ? 128 : 0), tmem_o = tmem_base + 256 + (second ? 128 : 0);
+      uint64_t *s_full = bars->s_full[second ? 1 : 0], *p_full = bars->p_full[second ? 1 : 0], *pv_done = bars->pv_done[second ? 1 : 0];
+      uint64_t *q_full = &bars->q_full[second ? 1 : 0], *o_free = &bars->o_free[second ? 1 : 0], *o_done = &bars->o_done[second ? 1 : 0];
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_word, p.a.err, code)); };
-      // parities, each flipped where a wait on it has been passed: buffers of K and V, score buffers, pieces of a query tile
-      uint32_t kb = 0, k_ph = 0, vb = 0, v_ph = 0;            // buffer, and its phase
-      uint32_t sb0 = 0, sb1 = 0, pb0 = 0, pb1 = 0, p_ph0 = 0, p_ph1 = 0;     // next score buffer; buffer of the next weights, and its phase
-      uint32_t q_ph0 = 0, q_ph1 = 0, o_ph0 = 1, o_ph1 = 1;
-      // S of the next keys into the next buffer of each query tile
-      auto scores_of = [&](uint64_t qd, uint64_t kd, uint32_t tmem, uint64_t* full) {
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < NC * 4; ++k)
-            umma_bf16(tmem, qd + static_cast<uint64_t>((k >> 2) * (16384 >> 4) + (k & 3) * 2), kd + static_cast<uint64_t>((k >> 2) * (8192 >> 4) + (k & 3) * 2), idesc_s,
-                      k > 0 ? 1u : 0u);
-          tc_commit(full);
-        }
-        __syncwarp();
-      };
-      auto scores = [&](bool two) {
+      // buffers, and their phases, each flipped where the buffer comes round: K, V, scores, weights; the queries and the accumulator have one
+      uint32_t kb = 0, k_ph = 0, vb = 0, v_ph = 0, sb = 0, pb = 0, p_ph = 0, q_ph = 0, o_ph = 1;
+      // S of the next keys into the next buffer (the product that read P of that buffer was issued before)
+      auto scores = [&](bool active) {
         wait(&bars->k_full[kb], k_ph, 752);
         if (!ok) return;
         tc_fence_after();
         const uint64_t kd = k_desc + static_cast<uint64_t>(kb * (Sh::kTile16 >> 4));
-        scores_of(q_desc, kd, tmem_base + sb0 * 64, &bars->s_full[0][sb0]);
-        sb0 ^= 1;
-        if (two) {
-          scores_of(q_desc + static_cast<uint64_t>(Sh::kQTile >> 4), kd, tmem_base + 128 + sb1 * 64, &bars->s_full[1][sb1]);
-          sb1 ^= 1;
+        const uint32_t to = tmem_s + sb * 64;
+        if (elect_one()) {
+          if (active) {
+#pragma unroll
+            for (int k = 0; k < NC * 4; ++k)
+              umma_bf16(to, q_desc + static_cast<uint64_t>((k >> 2) * (16384 >> 4) + (k & 3) * 2), kd + static_cast<uint64_t>((k >> 2) * (8192 >> 4) + (k & 3) * 2),
+                        idesc_s, k > 0 ? 1u : 0u);
+            tc_commit(&s_full[sb]);
+            tc_commit(&bars->k_empty[kb]);
+          } else {
+            mbar_arrive(&bars->k_empty[kb]);
+          }
         }
-        if (elect_one()) tc_commit(&bars->k_empty[kb]);
         __syncwarp();
+        if (active) sb ^= 1;
         kb ^= 1;
         k_ph ^= kb ^ 1;
-      };
-      auto product = [&](uint64_t vd, uint32_t tmem_o, uint32_t tmem_p, bool first, uint64_t* done, uint64_t* empty, uint64_t* all) {
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tmem_o, tmem_p + k * 8, vd + static_cast<uint64_t>(k * (2048 >> 4)), idesc_pv, (!first || k > 0) ? 1u : 0u);
-          tc_commit(done);
-          if (empty) tc_commit(empty);
-          if (all) tc_commit(all);
-        }
-        __syncwarp();
       };
       for (int i = 0; ok; ++i) {
         wait(&bars->piece_full[i % kPieces], (i / kPieces) & 1, 766);
         if (!ok) break;
         const Piece& pq = bars->piece[i % kPieces];
         const int nt = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(pq.nt < 0 ? 0 : pq.tb - pq.ta + 1))) - 1;
-        const bool two = __all_sync(0xffffffffu, pq.nt >= 0 && pq.two != 0);
+        const bool active = !second || __all_sync(0xffffffffu, pq.nt >= 0 && pq.two != 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->piece_empty[i % kPieces]);
         if (nt < 0) break;
-        wait(&bars->q_full[0], q_ph0, 762);
-        q_ph0 ^= 1;
-        if (two) { wait(&bars->q_full[1], q_ph1, 762); q_ph1 ^= 1; }
-        if (ok && nt > 0) scores(two);
+        if (active) { wait(q_full, q_ph, 762); q_ph ^= 1; }
+        if (ok && nt > 0) scores(active);
         for (int t = 0; t < nt && ok; ++t) {
-          if (t + 1 < nt) scores(two);              // the product that read P of that buffer was issued before
+          if (t + 1 < nt) scores(active);
           wait(&bars->v_full[vb], v_ph, 753);
+          if (active) {
+            if (t == 0) { wait(o_free, o_ph, 763); o_ph ^= 1; }
+            wait(&p_full[pb], p_ph, 754);
+          }
+          if (!ok) break;
+          tc_fence_after();
           const uint64_t vd = v_desc + static_cast<uint64_t>(vb * (Sh::kTile16 >> 4));
-          uint64_t* empty = &bars->v_empty[vb];
+          if (elect_one()) {
+            if (active) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16_ts(tmem_o, tmem_s + pb * 64 + k * 8, vd + static_cast<uint64_t>(k * (2048 >> 4)), idesc_pv, (t > 0 || k > 0) ? 1u : 0u);
+              tc_commit(&pv_done[pb]);
+              tc_commit(&bars->v_empty[vb]);
+              if (t + 1 == nt) tc_commit(o_done);
+            } else {
+              mbar_arrive(&bars->v_empty[vb]);
+            }
+          }
+          __syncwarp();
           vb ^= 1;
           v_ph ^= vb ^ 1;
-          if (t == 0) { wait(&bars->o_free[0], o_ph0, 763); o_ph0 ^= 1; }
-          wait(&bars->p_full[0][pb0], p_ph0, 754);
-          if (!ok) break;
-          product(vd, tmem_base + 256, tmem_base + pb0 * 64, t == 0, &bars->pv_done[0][pb0], two ? nullptr : empty, t + 1 == nt ? &bars->o_done[0] : nullptr);
-          pb0 ^= 1;
-          p_ph0 ^= pb0 ^ 1;
-          if (two) {
-            if (t == 0) { wait(&bars->o_free[1], o_ph1, 763); o_ph1 ^= 1; }
-            wait(&bars->p_full[1][pb1], p_ph1, 754);
-            if (!ok) break;
-            product(vd, tmem_base + 384, tmem_base + 128 + pb1 * 64, t == 0, &bars->pv_done[1][pb1], empty, t + 1 == nt ? &bars->o_done[1] : nullptr);
-            pb1 ^= 1;
-            p_ph1 ^= pb1 ^ 1;
-          }
+          if (active) { pb ^= 1; p_ph ^= pb ^ 1; }
         }
       }
     }
