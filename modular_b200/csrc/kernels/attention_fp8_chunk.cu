@@ -184,12 +184,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   if (tid == 0) {
     for (int s = 0; s < kRing; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 4); }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&bars->k_full[b], 4); mbar_init(&bars->k_empty[b], 2);
-      mbar_init(&bars->v_full[b], 4); mbar_init(&bars->v_empty[b], 2);
+      mbar_init(&bars->k_full[b], 2); mbar_init(&bars->k_empty[b], 2);
+      mbar_init(&bars->v_full[b], 2); mbar_init(&bars->v_empty[b], 2);
       for (int g = 0; g < 2; ++g) { mbar_init(&bars->s_full[g][b], 1); mbar_init(&bars->p_full[g][b], 4); mbar_init(&bars->pv_done[g][b], 1); }
       mbar_init(&bars->q_full[b], 4); mbar_init(&bars->o_done[b], 1); mbar_init(&bars->o_free[b], 4);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&bars->info_full[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars->info_full[i], 2);
     for (int i = 0; i < kPieces; ++i) { mbar_init(&bars->piece_full[i], 1); mbar_init(&bars->piece_empty[i], kRoles); }
     bars->abort_word = 0;
     fence_mbar_init();
@@ -386,14 +386,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    // ------------------------------------------------------------------ codes to f16
-    const int cw = warp - 12;
-    // 16 rows a warp, 16 codes a lane and step. With HD 128 the lanes of a quarter-warp take the first half of one row and the second half of its
+    // ------------------------------------------------------------------ codes to f16: warps 12 and 13 K, 14 and 15 V, 32 rows a warp. (Four warps on
+    // either in turn would hold the next keys up until the last product with V is through.)
+    const int cw = warp - 12, kv = cw >> 1;
+    // 16 codes a lane and step. With HD 128 the lanes of a quarter-warp take the first half of one row and the second half of its
     // neighbour: they read from all banks, and their writes, to the same places of two operand chunks, fall on different banks through the swizzle
-    const int chunk = NC == 2 ? (lane & 7) : (lane & 3), row0 = cw * 16 + (NC == 2 ? (lane >> 3) ^ (chunk >> 2) : lane >> 2);
-    constexpr int kSteps = NC * 2, kRowStep = 16 / kSteps;
+    const int chunk = NC == 2 ? (lane & 7) : (lane & 3), row0 = (cw & 1) * 32 + (NC == 2 ? (lane >> 3) ^ (chunk >> 2) : lane >> 2);
+    constexpr int kRowStep = NC == 2 ? 4 : 8, kSteps = 32 / kRowStep;
     const int piece = 2 * (chunk & 3);
     const uint32_t to_lo = (chunk >> 2) * 8192 + row0 * 128 + ((piece ^ (row0 & 7)) << 4), to_hi = to_lo ^ 16;
+    uint64_t *full16 = kv == 0 ? bars->k_full : bars->v_full, *empty16 = kv == 0 ? bars->k_empty : bars->v_empty;
+    uint8_t* tile16 = kv == 0 ? sK : sV;
     int s = 0, ct = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -405,79 +408,64 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->piece_empty[i % kPieces]);
       if (nt < 0) break;
-      for (int t = 0; t < nt && ok; ++t, ++ct) {
+      for (int t = 0; t < nt; ++t, ++ct) {
         const int b = ct & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[s], ph, abort_word, p.a.err, 755));
         if (!ok) break;
         const int n = bars->rows[s];
-        const uint8_t* sc = sScale + s * 128;
-        const uint8_t* from = sRing + s * Sh::kStage + row0 * HD + chunk * 16;
+        const uint8_t* sc = sScale + s * 128 + kv * 64;
+        const uint8_t* from = sRing + s * Sh::kStage + kv * Sh::kCodes + row0 * HD + chunk * 16;
         // all loads first: the stores that follow could not be told from them
-        uint4 code[2][kSteps];
-        int byte[2][kSteps], top[2];
+        uint4 code[kSteps];
+        int byte[kSteps];
+        const uint32_t two_bytes = *reinterpret_cast<const uint16_t*>(sc + 2 * lane);
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t two_bytes = *reinterpret_cast<const uint16_t*>(sc + kv * 64 + 2 * lane);
-          top[kv] = static_cast<int>(max(2 * lane < n ? two_bytes & 255u : 0u, 2 * lane + 1 < n ? two_bytes >> 8 : 0u));
+        for (int it = 0; it < kSteps; ++it) {
+          code[it] = *reinterpret_cast<const uint4*>(from + it * kRowStep * HD);
+          byte[it] = sc[row0 + it * kRowStep];
+        }
+        int top = static_cast<int>(__reduce_max_sync(0xffffffffu, max(2 * lane < n ? two_bytes & 255u : 0u, 2 * lane + 1 < n ? two_bytes >> 8 : 0u)));
+        if (kv == 1) top = min(max(top, kLeastByte), kMostByte);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->empty[s]);           // this warp's part of the stage is in registers
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty16[b], ((ct >> 1) & 1) ^ 1, abort_word, p.a.err, 756));
+        if (!ok) break;
+        // (the products of two tiles ago are through, so the softmax is done with what four tiles ago stood here)
+        if ((cw & 1) == 0 && lane == 0) {
+          if (kv == 0) bars->info[ct & 3].k = score_factor(p.a.scale * kLog2e, top - 127 - kHeadroom);
+          else bars->info[ct & 3].v = static_cast<float>(top - 127);
+          mbar_arrive(&bars->info_full[ct & 3]);
+        }
+        uint8_t* to = tile16 + b * Sh::kTile16;
+        if (n < 64) {                                // rows behind the last key become zeros
+#pragma unroll
+          for (int it = 0; it < kSteps; ++it)
+            if (row0 + it * kRowStep >= n) { code[it] = make_uint4(0, 0, 0, 0); byte[it] = 0; }
         }
 #pragma unroll
         for (int it = 0; it < kSteps; ++it) {
-          code[0][it] = *reinterpret_cast<const uint4*>(from + it * kRowStep * HD);
-          byte[0][it] = sc[row0 + it * kRowStep];
-        }
+          const uint32_t f = relative_scale(byte[it], top);
+          const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
+          const uint32_t words[4] = {code[it].x, code[it].y, code[it].z, code[it].w};
+          uint32_t h[8];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) top[kv] = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(top[kv])));
-        top[1] = min(max(top[1], kLeastByte), kMostByte);
-        if (warp == 12 && lane == 0) {
-          bars->info[ct & 3].k = score_factor(p.a.scale * kLog2e, top[0] - 127 - kHeadroom);
-          bars->info[ct & 3].v = static_cast<float>(top[1] - 127);
-          mbar_arrive(&bars->info_full[ct & 3]);
-        }
+          for (int k = 0; k < 4; ++k) {
+            uint32_t x[2];
+            codes_f16(words[k], x[0], x[1]);
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (kv == 1) {
-#pragma unroll
-            for (int it = 0; it < kSteps; ++it) {
-              code[1][it] = *reinterpret_cast<const uint4*>(from + Sh::kCodes + it * kRowStep * HD);
-              byte[1][it] = sc[64 + row0 + it * kRowStep];
+            for (int e = 0; e < 2; ++e) {
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), f2);
+              h[2 * k + e] = *reinterpret_cast<const uint32_t*>(&y);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->empty[s]);       // all of the stage is in registers
           }
-          ok = __all_sync(0xffffffffu, mbar_wait(kv == 0 ? &bars->k_empty[b] : &bars->v_empty[b], ((ct >> 1) & 1) ^ 1, abort_word, p.a.err, 756));
-          if (!ok) break;
-          uint8_t* to = (kv == 0 ? sK : sV) + b * Sh::kTile16;
-          if (n < 64) {                              // rows behind the last key become zeros
-#pragma unroll
-            for (int it = 0; it < kSteps; ++it)
-              if (row0 + it * kRowStep >= n) { code[kv][it] = make_uint4(0, 0, 0, 0); byte[kv][it] = 0; }
-          }
-#pragma unroll
-          for (int it = 0; it < kSteps; ++it) {
-            const uint32_t f = relative_scale(byte[kv][it], top[kv]);
-            const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
-            const uint4 c = code[kv][it];
-            const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-            uint32_t h[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t x[2];
-              codes_f16(words[k], x[0], x[1]);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), f2);
-                h[2 * k + e] = *reinterpret_cast<const uint32_t*>(&y);
-              }
-            }
-            // (four rows on the swizzle has another bit set: the place moves by 64 bytes the other way)
-            const uint32_t turn = NC == 2 ? (it & 1) << 6 : 0u;
-            *reinterpret_cast<uint4*>(to + ((to_lo ^ turn) + it * kRowStep * 128)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(to + ((to_hi ^ turn) + it * kRowStep * 128)) = make_uint4(h[4], h[5], h[6], h[7]);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(kv == 0 ? &bars->k_full[b] : &bars->v_full[b]);
+          // (four rows on the swizzle has another bit set: the place moves by 64 bytes the other way)
+          const uint32_t turn = NC == 2 ? (it & 1) << 6 : 0u;
+          *reinterpret_cast<uint4*>(to + ((to_lo ^ turn) + it * kRowStep * 128)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(to + ((to_hi ^ turn) + it * kRowStep * 128)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full16[b]);
         if (++s == kRing) { s = 0; ph ^= 1; }
       }
     }
