@@ -35,11 +35,13 @@ constexpr int kSetup = 2;               // units of a segment besides its tiles
 constexpr int kMinUnits = 6;            // of a share
 constexpr int kMaxTiles = 8192;         // plan tiles of a launch (their sums wait in shared memory)
 
+struct Cut;
+
 struct ChunkParams {
   MbFp8Attention a;
   MbFp8Cache c;
   float* ws;                            // [CTA][2][256][HD + 4]: O, m, l of a segment's piece that begins / ends a share
-  int* sums;                            // [n_tiles + 1], for join_chunks_kernel
+  Cut* cuts;                            // [CTA]: the segment whose first piece ends this CTA's share
   int box;
 };
 
@@ -51,6 +53,10 @@ struct Piece {
   int nt, ta, tb, head;                 // nt < 0: no more
   int seq, tq0, half_tok, two;          // two: the second MMA tile has rows
   int qs, ql, kl, kv_hi;
+};
+struct Cut {
+  int pieces;                           // 0: none
+  int head, tq0, half_tok, qs, ql, pad[2];
 };
 constexpr int kPieces = 4;
 constexpr int kRoles = 15;              // warps that take them: producer, two MMA issuers, four converters, eight of softmax
@@ -222,8 +228,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= n_tiles; i += kThreads) p.sums[i] = sums[i];
   const uint32_t tmem_base = bars->tmem_base;
   volatile int* abort_word = &bars->abort_word;
   const int64_t U = static_cast<int64_t>(run) * p.a.n_kv;
@@ -238,6 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       pc.u = cta < C ? chunk_start(U, C, cta) : 0;
       pc.end = cta < C ? chunk_start(U, C, cta + 1) : 0;
       bool more = true;
+      Cut cut = {};
       for (int i = 0; more; ++i) {
         more = pc.next(sums, n_tiles);
         Piece q;
@@ -248,11 +253,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           q.nt = pc.nt; q.ta = pc.ta; q.tb = pc.tb; q.head = pc.head;
           q.seq = w.seq; q.tq0 = w.tq0; q.half_tok = w.half_tok; q.two = w.two ? 1 : 0;
           q.qs = w.qs; q.ql = w.ql; q.kl = w.kl; q.kv_hi = w.kv_hi;
+          if (q.ta == 0 && q.tb < q.nt) {
+            const int64_t end = static_cast<int64_t>(q.head) * run + sums[pc.tile] + kSetup + q.nt - 1;
+            cut = Cut{chunk_holding(U, C, end) - cta + 1, q.head, q.tq0, q.half_tok, q.qs, q.ql, {0, 0}};
+          }
         }
         if (!mbar_wait(&bars->piece_empty[i % kPieces], ((i / kPieces) & 1) ^ 1, abort_word, p.a.err, 764)) break;
         bars->piece[i % kPieces] = q;
         mbar_arrive(&bars->piece_full[i % kPieces]);
       }
+      p.cuts[cta] = cut;
     } else if (warp == 0) {
       // ---------------------------------------------------------------- producer: places of the next 32 boxes by lane, a copy per lane
       // (one lane alone took 3250 cycles a tile, for the page number's round trip, the divisions and four copies)
@@ -652,54 +662,52 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   }
 }
 
-// Segments that lie in several shares. A block (times four, for 64 rows each) per border between two shares; the first border inside a segment adds its
-// pieces up, a warp per row in turn.
+// Segments that lie in several shares: blocks (CTA whose share ends with a segment's first piece, 32 rows), a warp per row. A lane per piece fetches
+// references and sums, then all pieces' values are on their way together.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) join_chunks_kernel(const __grid_constant__ ChunkParams p, int ctas) {
+__global__ void __launch_bounds__(512) join_chunks_kernel(const __grid_constant__ ChunkParams p) {
   pdl_wait();
   const MbFp8Attention& a = p.a;
-  const int n = a.n_tiles, per_head = p.sums[n], G = a.n_q / a.n_kv, border = blockIdx.x + 1;
-  const int64_t U = static_cast<int64_t>(per_head) * a.n_kv;
-  const int C = chunk_shares(U, ctas);
-  if (border >= C || U == 0) return;
-  const int64_t u = chunk_start(U, C, border);
-  const int head = static_cast<int>(u / per_head), v = static_cast<int>(u - static_cast<int64_t>(head) * per_head);
-  const int tile = tile_holding(p.sums, n, v);
-  const int len = p.sums[tile + 1] - p.sums[tile], nt = len - kSetup;
-  if (v - p.sums[tile] <= kSetup || nt <= 0) return;          // no tile of the segment lies before the border
-  const int64_t first = static_cast<int64_t>(head) * per_head + p.sums[tile] + kSetup;
-  const int c0 = chunk_holding(U, C, first), c1 = chunk_holding(U, C, first + nt - 1);
-  if (c0 != border - 1 || c0 == c1) return;                   // an earlier border's work
-  Work w;
-  if (!work_of(a, tile, w)) return;
-  const int lane = threadIdx.x & 31;
+  const Cut w = p.cuts[blockIdx.x];
+  if (w.pieces == 0) return;
+  const int G = a.n_q / a.n_kv, lane = threadIdx.x & 31;
   constexpr int PER = HD / 32;
   constexpr int64_t kSlot = 256 * (HD + 4);
-  for (int i = threadIdx.x >> 5; i < 64; i += 8) {
-    const int at = blockIdx.y * 64 + i, g = at >> 7, r = at & 127;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = blockIdx.y * 32 + i * 16 + (threadIdx.x >> 5), g = at >> 7, r = at & 127;
     const int tq = w.tq0 + g * w.half_tok + r / G;
     if (r >= w.half_tok * G || tq >= w.ql || w.qs + tq >= a.T) continue;
     // the first piece ends its share (slot 1), the others begin theirs (slot 0)
-    const float* row = p.ws + static_cast<int64_t>(c0) * 2 * kSlot + at * (HD + 4);
+    const float* row = p.ws + static_cast<int64_t>(blockIdx.x) * 2 * kSlot + at * (HD + 4);
     auto piece = [&](int k) { return row + (2 * k + (k == 0 ? 1 : 0)) * kSlot; };
-    const int pieces = c1 - c0 + 1;
-    float m = kNoMax;
-    for (int k = lane; k < pieces; k += 32) m = fmaxf(m, piece(k)[HD]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, o[PER];
+    float m = kNoMax, l = 0.f, o[PER];
 #pragma unroll
     for (int c = 0; c < PER; ++c) o[c] = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < pieces; ++k) {
-      const float* q = piece(k);
-      const float f = exp2f(q[HD] - m);
-      l = fmaf(q[HD + 1], f, l);
+    for (int k0 = 0; k0 < w.pieces; k0 += 32) {
+      const int n = min(32, w.pieces - k0);
+      const float mk = lane < n ? piece(k0 + lane)[HD] : kNoMax, lk = lane < n ? piece(k0 + lane)[HD + 1] : 0.f;
+      float top = fmaxf(m, mk);
 #pragma unroll
-      for (int c = 0; c < PER; ++c) o[c] = fmaf(q[lane * PER + c], f, o[c]);
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float keep = exp2f(m - top), f = exp2f(mk - top);
+      float sum = lk * f;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      l = l * keep + sum;
+      m = top;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) o[c] *= keep;
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float* q = piece(k0 + k) + lane * PER;
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+        for (int c = 0; c < PER; ++c) o[c] = fmaf(q[c], fk, o[c]);
+      }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(w.qs + tq) * a.ldo + static_cast<int64_t>(head * G + r % G) * HD + lane * PER;
+    T* dst = static_cast<T*>(a.out) + static_cast<int64_t>(w.qs + tq) * a.ldo + static_cast<int64_t>(w.head * G + r % G) * HD + lane * PER;
 #pragma unroll
     for (int c = 0; c < PER; ++c) dst[c] = static_cast<T>(o[c] * inv);
   }
@@ -708,7 +716,7 @@ __global__ void __launch_bounds__(256) join_chunks_kernel(const __grid_constant_
 static size_t slots_bytes(const MbFp8Attention& a, int num_sms) { return static_cast<size_t>(num_sms) * 2 * 256 * (a.head_dim + 4) * sizeof(float); }
 
 size_t chunk_workspace(const MbFp8Attention& a, int num_sms) {
-  return a.n_tiles > 0 ? slots_bytes(a, num_sms) + (min(a.n_tiles, kMaxTiles) + 1) * sizeof(int) : 0;
+  return a.n_tiles > 0 ? slots_bytes(a, num_sms) + num_sms * sizeof(Cut) : 0;
 }
 
 template <int HD, typename T>
@@ -726,7 +734,7 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
   ChunkParams p = {};
   p.c = c;
   p.ws = static_cast<float*>(a.ws);
-  p.sums = reinterpret_cast<int*>(static_cast<char*>(a.ws) + slots_bytes(a, num_sms));
+  p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.ws) + slots_bytes(a, num_sms));
   p.box = c.page_size % 64 == 0 ? 64 : c.page_size % 32 == 0 ? 32 : 16;
   for (int at = 0; at < a.n_tiles; at += kMaxTiles) {
     p.a = a;
@@ -735,7 +743,7 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
     p.a.n_tiles = min(kMaxTiles, a.n_tiles - at);
     const size_t smem = Shape<HD>::kSmem + (p.a.n_tiles + 1) * sizeof(int);
     if (launch_k(kern, dim3(num_sms), dim3(kThreads), smem, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
-    if (num_sms > 1 && launch_k(join_chunks_kernel<HD, T>, dim3(num_sms - 1, 4), dim3(256), 0, stream, p, num_sms) != cudaSuccess) return MB_ERR_LAUNCH;
+    if (launch_k(join_chunks_kernel<HD, T>, dim3(num_sms, 8), dim3(512), 0, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
   }
   return MB_OK;
 }

@@ -48,10 +48,16 @@ constexpr int kDecCtas = 2;             // per SM
 constexpr int kMinShare = 2;            // tiles
 constexpr int kMaxDecode = 4096;        // sequences of a launch (their tile counts wait in shared memory)
 
+// The sequence whose first piece ends a CTA's share
+struct DecCut {
+  int pieces, rows, qs, pad;            // pieces 0: none
+};
+
 struct DecParams {
   MbFp8Attention a;
   MbFp8Cache c;
   float* ws;
+  DecCut* cuts;              // [head][GX]
   int box, GX, rows_alloc;   // rows of a box; CTAs of a head; query rows kept in a partial result
 };
 
@@ -325,7 +331,11 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
       }
     }
   }
-  if (gx >= GE || U == 0) { pdl_trigger(); return; }
+  if (gx >= GE || U == 0) {
+    if (tid == 0) p.cuts[kvh * p.GX + gx] = DecCut{0, 0, 0, 0};
+    pdl_trigger();
+    return;
+  }
   const int u0 = share_start(U, GE, gx), u1 = share_start(U, GE, gx + 1);
   int first;                                        // the sequence that holds tile u0: the last i with prefix[i] <= u0
   {
@@ -344,6 +354,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
     int s = 0, n = 0;
     uint32_t ph = 0;
     bool ok = true;
+    DecCut cut = {0, 0, 0, 0};
     for (int i = first, u = u0; u < u1 && ok; ++i) {
       const int fu = prefix[i], t1 = min(prefix[i + 1], u1) - fu;
       if (t1 <= u - fu) continue;
@@ -354,6 +365,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
       if (ql * G > 8 * NR && lane == 0 && p.a.err) atomicCAS(p.a.err, 0, 732);        // (not a plan of these sequences)
       ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_empty, (n & 1) ^ 1, abort_word, p.a.err, 743));
       if (!ok) break;
+      if (u == fu && t1 < prefix[i + 1] - fu) cut = DecCut{share_holding(U, GE, prefix[i + 1] - 1) - gx + 1, rows, qs, 0};
       {
         const int row = qs + lane / G;
         const bool there = lane < rows && row < p.a.T;
@@ -402,6 +414,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
       }
       u = fu + t1;
     }
+    if (lane == 0) p.cuts[kvh * p.GX + gx] = cut;
     pdl_trigger();
     return;
   }
@@ -532,42 +545,22 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
   }
 }
 
-// Sequences that lie in several shares: a block per (sequence, head) finds them by the same sums and adds the pieces up. First every piece's
-// weight, then four groups of 128 threads take pieces in turn (one after the other they would cost a round trip to L2 each).
+// Sequences that lie in several shares: a block per CTA whose share ends with a sequence's first piece. First every piece's weight, then four groups of 128
+// threads take pieces in turn (one after the other they would cost a round trip to L2 each).
 template <int HD, typename T>
 __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ DecParams p) {
   constexpr int kPieces = 64;                        // weights kept at a time
-  __shared__ int part[16], part_all[16];
   __shared__ float weight[kPieces][16], share[kPieces][16], total[2][16];     // of a piece's values, and times its sum
   __shared__ float4 sum[3][128];
   pdl_wait();
-  const int i = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, nd = p.a.n_decode, G = p.a.n_q / p.a.n_kv;
-  const int nt = tiles_of(p.a, i);
-  int before = 0, all = 0;
-  for (int k = tid; k < nd; k += 512) {
-    const int n = tiles_of(p.a, k);
-    all += n;
-    if (k < i) before += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if ((tid & 31) == 0) { part[tid >> 5] = before; part_all[tid >> 5] = all; }
-  __syncthreads();
-  int fu = 0, U = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) { fu += part[w]; U += part_all[w]; }
-  if (nt == 0) return;
-  const int GE = shares_of(U, p.GX), g0 = share_holding(U, GE, fu), g1 = share_holding(U, GE, fu + nt - 1);
-  if (g0 == g1) return;                              // finished by its CTA
-  const int seq = p.a.decode_seq[i], qs = p.a.q_start[seq], rows = min(p.a.q_len[seq] * G, 16);
+  const int kvh = blockIdx.y, tid = threadIdx.x, G = p.a.n_q / p.a.n_kv;
+  const DecCut cut = p.cuts[kvh * p.GX + blockIdx.x];
+  if (cut.pieces == 0) return;
+  const int qs = cut.qs, rows = cut.rows, n = cut.pieces, group = tid >> 7, lane = tid & 127, half = lane >> 4, r16 = lane & 15;
   // a piece lies in slot 0 of its CTA, the first one, where the sequence begins, in slot 1
   const int64_t slot = slot_floats<HD>(p.rows_alloc);
-  const float* base = p.ws + (static_cast<int64_t>(kvh) * p.GX + g0) * 2 * slot;
+  const float* base = p.ws + (static_cast<int64_t>(kvh) * p.GX + blockIdx.x) * 2 * slot;
   auto slot_of = [&](int k) { return base + (2 * k + (k == 0 ? 1 : 0)) * slot; };
-  const int n = g1 - g0 + 1, group = tid >> 7, lane = tid & 127, half = lane >> 4, r16 = lane & 15;
   // the largest reference of each row
   if (group == 0) {
     float m = kNoMax;
@@ -629,7 +622,7 @@ static int decode_ctas(int n_kv, int num_sms) { return max(1, kDecCtas * num_sms
 
 size_t decode_workspace(int n_decode, int n_q, int n_kv, int head_dim, int num_sms) {
   if (n_decode <= 0) return 0;
-  return static_cast<size_t>(n_kv) * decode_ctas(n_kv, num_sms) * 2 * (16 * head_dim + 32) * sizeof(float);
+  return static_cast<size_t>(n_kv) * decode_ctas(n_kv, num_sms) * (2 * (16 * head_dim + 32) * sizeof(float) + sizeof(DecCut));
 }
 
 template <int HD, int NR, typename T>
@@ -648,6 +641,7 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
   p.GX = decode_ctas(a.n_kv, num_sms);
   p.rows_alloc = 16;
   p.ws = static_cast<float*>(a.ws);
+  p.cuts = reinterpret_cast<DecCut*>(p.ws + static_cast<size_t>(a.n_kv) * p.GX * 2 * slot_floats<HD>(16));
   CUtensorMap tk, tv;
   auto map = [&](CUtensorMap* m, const void* base, long long head, long long page) {
     const uint64_t h = a.n_kv > 1 ? head : static_cast<uint64_t>(c.page_size) * HD;
@@ -662,7 +656,7 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
     p.a.n_decode = min(kMaxDecode, a.n_decode - at);
     const size_t smem = fixed + (p.a.n_decode + 1) * sizeof(int);
     if (launch_k(kern, dim3(p.GX, a.n_kv), dim3(Team<NR>::kThreads), smem, stream, tk, tv, p) != cudaSuccess) return MB_ERR_LAUNCH;
-    if (launch_k(join_kernel<HD, T>, dim3(p.a.n_decode, a.n_kv), dim3(512), 0, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
+    if (launch_k(join_kernel<HD, T>, dim3(p.GX, a.n_kv), dim3(512), 0, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
   }
   return MB_OK;
 }
