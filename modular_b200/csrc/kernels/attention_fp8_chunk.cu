@@ -32,8 +32,8 @@ constexpr int kRing = 3;                // stages of codes
 constexpr int kThreads = 512;
 constexpr int kHeadroom = 6;            // the tile's largest scale becomes 2^6: codes reach 2^15 of f16
 constexpr int kSetup = 2;               // units of a segment besides its tiles
-constexpr int kMinUnits = 6;            // of a share
-constexpr int kMaxTiles = 8192;         // plan tiles of a launch (their sums wait in shared memory)
+constexpr int kMinUnits = 3;            // of a share
+constexpr int kMaxTiles = 2048;         // plan tiles of a launch (their sums wait in shared memory)
 
 struct Cut;
 
@@ -83,7 +83,8 @@ struct Shape {
   static constexpr int kCodes = 64 * HD;
   static constexpr int kStage = 2 * kCodes;
   static constexpr int kTile16 = NC * 64 * 128;                   // an operand tile
-  static constexpr size_t kSmem = 2 * kQTile + 4 * kTile16 + kRing * (kStage + 128) + sizeof(ChunkBars);
+  static constexpr int kTurn = 32 * 128;                           // a warp's 32 rows x 32 columns on their way out
+  static constexpr size_t kSmem = 2 * kQTile + 4 * kTile16 + kRing * (kStage + 128) + 8 * kTurn + sizeof(ChunkBars);
 };
 
 // MN-major operand with 128B swizzle: see attention_tc.cu
@@ -132,10 +133,17 @@ __device__ __forceinline__ bool work_of(const MbFp8Attention& a, int tile, Work&
   return w.tq0 < w.ql;
 }
 
-// CTAs that get work, and the first unit of CTA c's share; U < 2^31
-__device__ __forceinline__ int chunk_shares(int64_t U, int ctas) { return static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(ctas), U / kMinUnits))); }
-__device__ __forceinline__ int64_t chunk_start(int64_t U, int C, int c) { return U * c / C; }
-__device__ __forceinline__ int chunk_holding(int64_t U, int C, int64_t u) { return static_cast<int>(((u + 1) * C - 1) / U); }
+// Of U units every one of C CTAs gets U / C, the first U % C one more. (32 bits: a billion units are 2^36 keys.)
+struct Shares {
+  int C, each, more;
+  __device__ __forceinline__ Shares(int U, int ctas) {
+    C = max(1, min(ctas, U / kMinUnits));
+    each = U / C;
+    more = U - each * C;
+  }
+  __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
+  __device__ __forceinline__ int holding(int u) const { return u < (each + 1) * more ? u / (each + 1) : more + (u - (each + 1) * more) / each; }
+};
 // the tile whose units hold v: the last one whose sum is at most v
 __device__ __forceinline__ int tile_holding(const int* sums, int n, int v) {
   int lo = 0, hi = n - 1;
@@ -148,16 +156,15 @@ __device__ __forceinline__ int tile_holding(const int* sums, int n, int v) {
 
 // The pieces of a CTA's share, in order
 struct Pieces {
-  int64_t u, end;
-  int head, tile, nt, ta, tb;
+  int u, end, head, tile, nt, ta, tb;
   __device__ __forceinline__ bool next(const int* sums, int n) {
     const int per_head = sums[n];
     while (u < end) {
-      head = static_cast<int>(u / per_head);
-      const int v = static_cast<int>(u - static_cast<int64_t>(head) * per_head);
+      head = u / per_head;
+      const int v = u - head * per_head;
       tile = tile_holding(sums, n, v);
       const int a = v - sums[tile], len = sums[tile + 1] - sums[tile];
-      const int b = static_cast<int>(min(static_cast<int64_t>(len), a + (end - u)));
+      const int b = min(len, a + (end - u));
       u += b - a;
       nt = len - kSetup;
       ta = max(0, a - kSetup);
@@ -182,7 +189,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   uint8_t* sV = sK + 2 * Sh::kTile16;
   uint8_t* sRing = sV + 2 * Sh::kTile16;            // [stage][K codes | V codes]
   uint8_t* sScale = sRing + kRing * Sh::kStage;     // [stage][K 64 | V 64]
-  ChunkBars* bars = reinterpret_cast<ChunkBars*>(sScale + kRing * 128);
+  uint8_t* sTurn = sScale + kRing * 128;            // [softmax warp][32 rows x 128 B]
+  ChunkBars* bars = reinterpret_cast<ChunkBars*>(sTurn + 8 * Sh::kTurn);
   int* sums = reinterpret_cast<int*>(bars + 1);     // [n_tiles + 1]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.a.n_q / p.a.n_kv, n_tiles = p.a.n_tiles;
@@ -230,8 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
   volatile int* abort_word = &bars->abort_word;
-  const int64_t U = static_cast<int64_t>(run) * p.a.n_kv;
-  const int C = chunk_shares(U, gridDim.x), cta = blockIdx.x;
+  const int cta = blockIdx.x;
 
   // 512 x 128 registers at launch = 128 x (88 + 160 + 160 + 104)
   if (warp < 4) {
@@ -239,8 +246,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     if (warp == 2 && lane == 0) {
       // ---------------------------------------------------------------- pieces
       Pieces pc;
-      pc.u = cta < C ? chunk_start(U, C, cta) : 0;
-      pc.end = cta < C ? chunk_start(U, C, cta + 1) : 0;
+      const Shares shares(run * p.a.n_kv, gridDim.x);
+      pc.u = cta < shares.C ? shares.start(cta) : 0;
+      pc.end = cta < shares.C ? shares.start(cta + 1) : 0;
       bool more = true;
       Cut cut = {};
       for (int i = 0; more; ++i) {
@@ -254,8 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           q.seq = w.seq; q.tq0 = w.tq0; q.half_tok = w.half_tok; q.two = w.two ? 1 : 0;
           q.qs = w.qs; q.ql = w.ql; q.kl = w.kl; q.kv_hi = w.kv_hi;
           if (q.ta == 0 && q.tb < q.nt) {
-            const int64_t end = static_cast<int64_t>(q.head) * run + sums[pc.tile] + kSetup + q.nt - 1;
-            cut = Cut{chunk_holding(U, C, end) - cta + 1, q.head, q.tq0, q.half_tok, q.qs, q.ql, {0, 0}};
+            cut = Cut{shares.holding(q.head * run + sums[pc.tile + 1] - 1) - cta + 1, q.head, q.tq0, q.half_tok, q.qs, q.ql, {0, 0}};
           }
         }
         if (!mbar_wait(&bars->piece_empty[i % kPieces], ((i / kPieces) & 1) ^ 1, abort_word, p.a.err, 764)) break;
@@ -487,34 +494,36 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     bool ok = true;
     int ct = 0, cg = 0, done = 0;                    // tiles so far: all, and of this query tile; its pieces that had tiles
     int at = 0, qe = 0;                              // the piece whose queries are in place, and their exponent
-    // this thread's query row of the piece, in f16 with the 128-byte swizzle, the largest value in [2^14, 2^15)
+    // the warp's 32 query rows of the piece, in f16 with the 128-byte swizzle, each row's largest value in [2^14, 2^15). HD / 8 lanes read a row together
     auto bring_queries = [&]() {
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->piece_full[at % kPieces], (at / kPieces) & 1, abort_word, p.a.err, 768));
       if (!ok) return;
       const Piece& w = bars->piece[at % kPieces];
       if (w.nt < 0 || (g == 1 && !w.two)) return;
+      constexpr int LPR = HD / 8, RPI = 32 / LPR, kIts = 32 / RPI;             // lanes of a row, rows and number of a step
       const int tq = w.tq0 + g * w.half_tok + r / G;
       const bool valid = r < w.half_tok * G && tq < w.ql && w.qs + tq < p.a.T;
-      const T* src = static_cast<const T*>(p.a.q) + static_cast<int64_t>(valid ? w.qs + tq : 0) * p.a.ldq + static_cast<int64_t>(w.head * G + r % G) * HD;
-      uint4 raw[HD / 8];
+      const int64_t mine = valid ? static_cast<int64_t>(w.qs + tq) * p.a.ldq + static_cast<int64_t>(w.head * G + r % G) * HD : -1;
+      uint4 raw[kIts];
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) raw[c] = valid ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
-      float big = 0.f;
+      for (int it = 0; it < kIts; ++it) {
+        const int64_t from = __shfl_sync(0xffffffffu, mine, it * RPI + lane / LPR);
+        raw[it] = from >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + from + (lane % LPR) * 8) : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) {
-        float x[8];
-        widen8<T>(raw[c], x);
+      for (int it = 0; it < kIts; ++it) {
+        float x[8], big = 0.f;
+        widen8<T>(raw[it], x);
 #pragma unroll
         for (int k = 0; k < 8; ++k) big = fmaxf(big, finite_abs(x[k]));
-      }
-      qe = f16_shift(big);
-      const float mul = pow2f(qe);
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) {
-        float x[8];
-        widen8<T>(raw[c], x);
-        uint8_t* row = sQ + g * Sh::kQTile + (c >> 3) * 16384 + r * 128;
-        *reinterpret_cast<uint4*>(row + (((c & 7) ^ (r & 7)) << 4)) =
+        for (int o = LPR / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        const int e = f16_shift(big);
+        const float mul = pow2f(e);
+        const int theirs = __shfl_sync(0xffffffffu, e, (lane % RPI) * LPR);    // of row it * RPI + lane % RPI
+        if (lane / RPI == it) qe = theirs;
+        const int row = quad * 32 + it * RPI + lane / LPR, c = lane % LPR;
+        *reinterpret_cast<uint4*>(sQ + g * Sh::kQTile + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
             make_uint4(pack_f16(x[0] * mul, x[1] * mul), pack_f16(x[2] * mul, x[3] * mul), pack_f16(x[4] * mul, x[5] * mul), pack_f16(x[6] * mul, x[7] * mul));
       }
       fence_proxy_async_smem();
@@ -623,9 +632,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         tc_fence_after();
       }
       const float f = (whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f) * (1.f / (1 << kHeadroom));
-      T* orow = static_cast<T*>(p.a.out) + static_cast<int64_t>(my_row ? row : 0) * p.a.ldo + static_cast<int64_t>(head) * HD;
-      // a piece that begins its CTA's share goes to slot 0, one that ends it to slot 1
+      // 32 columns at a time turn round in shared memory, so that eight lanes write a row together. A piece that begins its CTA's share goes to slot 0,
+      // one that ends it to slot 1
       float* part = p.ws + ((static_cast<int64_t>(cta) * 2 + (ta > 0 ? 0 : 1)) * 256 + g * 128 + r) * (HD + 4);
+      const int64_t place = my_row ? static_cast<int64_t>(row) * p.a.ldo + static_cast<int64_t>(head) * HD : -1;
+      uint8_t* turn = sTurn + (warp - 4) * Sh::kTurn;
 #pragma unroll
       for (int q4 = 0; q4 < HD / 32; ++q4) {
         uint32_t tr[32];
@@ -636,13 +647,21 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
           for (int c = 0; c < 32; ++c) tr[c] = 0;
         }
-        if (my_row) {
+        __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 v = make_float4(__uint_as_float(tr[c]), __uint_as_float(tr[c + 1]), __uint_as_float(tr[c + 2]), __uint_as_float(tr[c + 3]));
-            if (whole) store4(orow + q4 * 32 + c, v, f);
-            else *reinterpret_cast<float4*>(part + q4 * 32 + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-          }
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<float4*>(turn + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+              make_float4(__uint_as_float(tr[4 * c]) * f, __uint_as_float(tr[4 * c + 1]) * f, __uint_as_float(tr[4 * c + 2]) * f, __uint_as_float(tr[4 * c + 3]) * f);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int rr = j * 4 + (lane >> 3);
+          const float4 v = *reinterpret_cast<const float4*>(turn + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+          const int64_t to = __shfl_sync(0xffffffffu, place, rr);
+          if (to < 0) continue;
+          const int col = q4 * 32 + (lane & 7) * 4;
+          if (whole) store4(static_cast<T*>(p.a.out) + to + col, v, 1.f);
+          else *reinterpret_cast<float4*>(part + (rr - lane) * (HD + 4) + col) = v;
         }
       }
       if (my_row && !whole) { part[HD] = unset ? kNoMax : m; part[HD + 1] = l; }
@@ -728,6 +747,9 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
     cudaFuncAttributes at;
     if (cudaFuncGetAttributes(&at, kern) != cudaSuccess || at.numRegs != 128) return MB_ERR_LAUNCH;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<HD>::kSmem + (kMaxTiles + 1) * sizeof(int))) != cudaSuccess)
+      return MB_ERR_LAUNCH;
+    // the same split of an SM's memory as the kernel it follows: changing it would drain the SM first
+    if (cudaFuncSetAttribute(join_chunks_kernel<HD, T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
       return MB_ERR_LAUNCH;
     configured.done();
   }

@@ -633,6 +633,9 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
   if (configured.needed()) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(fixed + (kMaxDecode + 1) * sizeof(int))) != cudaSuccess)
       return MB_ERR_LAUNCH;
+    // the same split of an SM's memory as the kernel it follows: changing it would drain the SM first
+    if (cudaFuncSetAttribute(join_kernel<HD, T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+      return MB_ERR_LAUNCH;
     configured.done();
   }
   DecParams p = {};
