@@ -87,6 +87,16 @@ __device__ __forceinline__ void widen8(uint4 r, float (&x)[8]) {
     x[2 * i] = f.x; x[2 * i + 1] = f.y;
   }
 }
+template <typename T>
+__device__ __forceinline__ float to_float(uint32_t bits) {
+  if constexpr (__is_same(T, __half)) return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  else return __uint_as_float(bits << 16);
+}
+// 16 bytes to shared memory, or zeros where `there` is false; copies_wait() waits for all of this thread's
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // 16 consecutive values (32 bytes, 16-byte aligned)
 template <typename T>
 __device__ __forceinline__ void load16(const T* src, float (&x)[16], bool valid) {

@@ -1,7 +1,7 @@
 // Attention of chunks of new tokens over the 8-bit paged cache, on the 5th-generation tensor cores.
 //
 // A segment is 256 query rows of one (sequence, key/value head): two MMA tiles of 128, tokens x the query heads that share the head, against the keys they
-// see, 64 at a time. All segments are one line of work (their tiles, and two units each for what a segment costs besides), cut into equal shares for one
+// see, 64 at a time. All segments are one line of work (their tiles, and some units each for what a segment costs besides), cut into equal shares for one
 // CTA per SM. A segment that is cut leaves partial results, which join_chunks_kernel adds up.
 //
 //   warp 2        walks over the share and hands its pieces to the others
@@ -31,8 +31,8 @@ namespace a8 {
 constexpr int kRing = 3;                // stages of codes
 constexpr int kThreads = 512;
 constexpr int kHeadroom = 6;            // the tile's largest scale becomes 2^6: codes reach 2^15 of f16
-constexpr int kSetup = 2;               // units of a segment besides its tiles
-constexpr int kMinUnits = 3;            // of a share
+constexpr int kSetup = 4;               // units of a segment besides its tiles: bringing its queries and results in and out takes that long
+constexpr int kMinUnits = kSetup + 1;   // of a share
 constexpr int kMaxTiles = 2048;         // plan tiles of a launch (their sums wait in shared memory)
 
 struct Cut;
@@ -494,37 +494,52 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     bool ok = true;
     int ct = 0, cg = 0, done = 0;                    // tiles so far: all, and of this query tile; its pieces that had tiles
     int at = 0, qe = 0;                              // the piece whose queries are in place, and their exponent
-    // the warp's 32 query rows of the piece, in f16 with the 128-byte swizzle, each row's largest value in [2^14, 2^15). HD / 8 lanes read a row together
+    // the warp's 32 query rows of the piece, in f16 with the 128-byte swizzle, each row's largest value in [2^14, 2^15). HD / 8 lanes fetch a row together
     auto bring_queries = [&]() {
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->piece_full[at % kPieces], (at / kPieces) & 1, abort_word, p.a.err, 768));
       if (!ok) return;
       const Piece& w = bars->piece[at % kPieces];
       if (w.nt < 0 || (g == 1 && !w.two)) return;
-      constexpr int LPR = HD / 8, RPI = 32 / LPR, kIts = 32 / RPI;             // lanes of a row, rows and number of a step
+      constexpr int LPR = HD / 8, RPI = 32 / LPR;    // lanes of a row, rows of a step
       const int tq = w.tq0 + g * w.half_tok + r / G;
       const bool valid = r < w.half_tok * G && tq < w.ql && w.qs + tq < p.a.T;
       const int64_t mine = valid ? static_cast<int64_t>(w.qs + tq) * p.a.ldq + static_cast<int64_t>(w.head * G + r % G) * HD : -1;
-      uint4 raw[kIts];
-#pragma unroll
-      for (int it = 0; it < kIts; ++it) {
-        const int64_t from = __shfl_sync(0xffffffffu, mine, it * RPI + lane / LPR);
-        raw[it] = from >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + from + (lane % LPR) * 8) : make_uint4(0, 0, 0, 0);
+      // As they are into their places, then each thread turns its own row into f16 there. (Loops that stay loops: this runs once a piece, and fetching
+      // straight code for it took longer than running it.)
+      uint8_t* tile = sQ + g * Sh::kQTile + quad * 32 * 128;
+#pragma unroll 2
+      for (int i = 0; i < 32; i += RPI) {
+        const int row = i + lane / LPR, c = lane % LPR;
+        const int64_t from = __shfl_sync(0xffffffffu, mine, row);
+        copy16_async(smem_u32(tile + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4)), static_cast<const T*>(p.a.q) + (from >= 0 ? from + c * 8 : 0), from >= 0);
       }
+      copies_wait();
+      __syncwarp();
+      uint32_t big2 = 0;                             // magnitudes of 16-bit floats order as integers do
+#pragma unroll 4
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 x = *reinterpret_cast<const uint4*>(tile + (c >> 3) * 16384 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4));
+        big2 = __vmaxu2(big2, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+      }
+      float big = to_float<T>(max(big2 & 0xffffu, big2 >> 16));
+      if (!(big < INFINITY)) {                       // leave out what is not finite
+        big = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < HD / 8; ++c) {
+          float x[8];
+          widen8<T>(*reinterpret_cast<const uint4*>(tile + (c >> 3) * 16384 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)), x);
 #pragma unroll
-      for (int it = 0; it < kIts; ++it) {
-        float x[8], big = 0.f;
-        widen8<T>(raw[it], x);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) big = fmaxf(big, finite_abs(x[k]));
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        const int e = f16_shift(big);
-        const float mul = pow2f(e);
-        const int theirs = __shfl_sync(0xffffffffu, e, (lane % RPI) * LPR);    // of row it * RPI + lane % RPI
-        if (lane / RPI == it) qe = theirs;
-        const int row = quad * 32 + it * RPI + lane / LPR, c = lane % LPR;
-        *reinterpret_cast<uint4*>(sQ + g * Sh::kQTile + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-            make_uint4(pack_f16(x[0] * mul, x[1] * mul), pack_f16(x[2] * mul, x[3] * mul), pack_f16(x[4] * mul, x[5] * mul), pack_f16(x[6] * mul, x[7] * mul));
+          for (int k = 0; k < 8; ++k) big = fmaxf(big, finite_abs(x[k]));
+        }
+      }
+      qe = f16_shift(big);                           // the largest goes into [2^14, 2^15)
+      const float mul = pow2f(qe);
+#pragma unroll 2
+      for (int c = 0; c < HD / 8; ++c) {
+        uint4* at16 = reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4));
+        float x[8];
+        widen8<T>(*at16, x);
+        *at16 = make_uint4(pack_f16(x[0] * mul, x[1] * mul), pack_f16(x[2] * mul, x[3] * mul), pack_f16(x[4] * mul, x[5] * mul), pack_f16(x[6] * mul, x[7] * mul));
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -637,7 +652,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       float* part = p.ws + ((static_cast<int64_t>(cta) * 2 + (ta > 0 ? 0 : 1)) * 256 + g * 128 + r) * (HD + 4);
       const int64_t place = my_row ? static_cast<int64_t>(row) * p.a.ldo + static_cast<int64_t>(head) * HD : -1;
       uint8_t* turn = sTurn + (warp - 4) * Sh::kTurn;
+      int64_t places[8];
 #pragma unroll
+      for (int j = 0; j < 8; ++j) places[j] = __shfl_sync(0xffffffffu, place, j * 4 + (lane >> 3));
+#pragma unroll 1
       for (int q4 = 0; q4 < HD / 32; ++q4) {
         uint32_t tr[32];
         if (nt > 0) {
@@ -657,11 +675,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         for (int j = 0; j < 8; ++j) {
           const int rr = j * 4 + (lane >> 3);
           const float4 v = *reinterpret_cast<const float4*>(turn + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-          const int64_t to = __shfl_sync(0xffffffffu, place, rr);
-          if (to < 0) continue;
           const int col = q4 * 32 + (lane & 7) * 4;
-          if (whole) store4(static_cast<T*>(p.a.out) + to + col, v, 1.f);
-          else *reinterpret_cast<float4*>(part + (rr - lane) * (HD + 4) + col) = v;
+          if (places[j] >= 0) {
+            if (whole) store4(static_cast<T*>(p.a.out) + places[j] + col, v, 1.f);
+            else *reinterpret_cast<float4*>(part + (rr - lane) * (HD + 4) + col) = v;
+          }
         }
       }
       if (my_row && !whole) { part[HD] = unset ? kNoMax : m; part[HD + 1] = l; }
