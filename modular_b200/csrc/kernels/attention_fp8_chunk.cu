@@ -31,7 +31,7 @@ namespace a8 {
 constexpr int kRing = 3;                // stages of codes
 constexpr int kThreads = 512;
 constexpr int kHeadroom = 6;            // the tile's largest scale becomes 2^6: codes reach 2^15 of f16
-constexpr int kSetup = 4;               // units of a segment besides its tiles: bringing its queries and results in and out takes that long
+constexpr int kSetup = 5;               // units of a segment besides its tiles: bringing its queries and results in and out takes that long
 constexpr int kMinUnits = kSetup + 1;   // of a share
 constexpr int kMaxTiles = 2048;         // plan tiles of a launch (their sums wait in shared memory)
 

@@ -505,15 +505,18 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
       }
     // a piece that begins its CTA's share goes to slot 0, one that ends it to slot 1
     float* slot = p.ws + (static_cast<int64_t>(kvh * p.GX + gx) * 2 + (w.ta > 0 ? 0 : 1)) * slot_floats<HD>(p.rows_alloc);
-#pragma unroll
-    for (int r0 = 0; r0 < 8 * NR; r0 += 2) {
-      if (r0 >= w.rows) break;
+    // (a loop that stays one: fetching straight code that runs once a piece takes longer than running it)
+#pragma unroll 1
+    for (int r0 = 0; r0 < w.rows; r0 += 2) {
       if (t4 == (r0 & 7) >> 1) {
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float2*>(sO + (warp * 2 + e) * (HD + 4) + c * 16 + 2 * g) = make_float2(st.o[c][r0 >> 3][e], st.o[c][r0 >> 3][2 + e]);
+          for (int e = 0; e < 2; ++e) {
+            const bool up = NR == 2 && r0 >= 8;
+            *reinterpret_cast<float2*>(sO + (warp * 2 + e) * (HD + 4) + c * 16 + 2 * g) =
+                make_float2(up ? st.o[c][NR - 1][e] : st.o[c][0][e], up ? st.o[c][NR - 1][2 + e] : st.o[c][0][2 + e]);
+          }
       }
       consumers_sync<kWorkers>();
       if (tid < HD / 2) {                            // 2 rows of HD / 4 pieces
