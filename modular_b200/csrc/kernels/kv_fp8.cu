@@ -30,16 +30,29 @@ struct Pack8 {
   T v[8];
 };
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  __align__(16) Pack8<T> r;
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
-  } else {
-    reinterpret_cast<uint4*>(&r)[0] = reinterpret_cast<const uint4*>(p)[0];
-    reinterpret_cast<uint4*>(&r)[1] = reinterpret_cast<const uint4*>(p)[1];
-  }
+struct Raw8 {                            // eight values as they lie in memory
+  uint4 r[sizeof(T) / 2];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(r.v[i]);
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void widen(float (&x)[8]) const {
+    __align__(16) Pack8<T> v;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(&v)[i] = r[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(v.v[i]);
+  }
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  Raw8<T> r;
+  r.load(p);
+  r.widen(x);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
@@ -199,7 +212,7 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreParams p) {
 // pairs, or two neighbouring groups. A warp takes one token and walks over some of its rows, 32 / LANES at a time, with the angles in registers: they
 // are read once for all heads (a thread an element group with its own angles: 108 us for 8192 tokens of 32 + 2 x 8 heads of 128).
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) store_rows_kernel(const StoreParams p, int per_warp) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) store_rows_kernel(const StoreParams p, int per_warp) {
   constexpr int LANES = HD / 16, RPW = 32 / LANES;
   pdl_wait();
   const int rows = p.n_q + 2 * p.n_kv, lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES;
@@ -213,6 +226,22 @@ __global__ void __launch_bounds__(256) store_rows_kernel(const StoreParams p, in
   const int a0 = p.interleaved ? part * 16 : lanes_turn ? part * 8 : p.rot + (part * 8 - half) * 2;
   const int b0 = p.interleaved ? a0 + 8 : lanes_turn ? a0 + half : a0 + 8;
   const bool turn_a = p.interleaved ? a0 < p.rot : lanes_turn, turn_b = p.interleaved ? b0 < p.rot : lanes_turn;
+  const T* src = static_cast<const T*>(p.qkv) + static_cast<int64_t>(t) * p.ld;
+  T* dst = static_cast<T*>(p.q_out) + static_cast<int64_t>(t) * p.ldq;
+  // the first rows are on their way before the angles, and each step's while those before it are worked on
+  constexpr int kAhead = 2;
+  Raw8<T> raw[kAhead][2];
+  auto fetch = [&](int h, Raw8<T> (&to)[2]) {
+    if (h < h1) {
+      to[0].load(src + static_cast<int64_t>(h) * HD + a0);
+      to[1].load(src + static_cast<int64_t>(h) * HD + b0);
+    } else {
+      to[0].clear();
+      to[1].clear();
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) fetch(h0 + sub + u * RPW, raw[u]);
   float c[8], s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) { c[i] = 1.f; s[i] = 0.f; }
@@ -239,26 +268,15 @@ __global__ void __launch_bounds__(256) store_rows_kernel(const StoreParams p, in
     }
     if (slot >= 0) { page = slot / p.c.page_size; off = static_cast<int>(slot - page * p.c.page_size); }
   }
-  const T* src = static_cast<const T*>(p.qkv) + static_cast<int64_t>(t) * p.ld;
-  T* dst = static_cast<T*>(p.q_out) + static_cast<int64_t>(t) * p.ldq;
-  // two steps of rows at a time: the second's loads are in flight while the first is worked on
-  for (int hb = h0 + sub; hb - sub < h1; hb += 2 * RPW) {
-    float x[2][2][8];
+#pragma unroll 1
+  for (int hb = h0 + sub; hb - sub < h1; hb += kAhead * RPW) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kAhead; ++u) {
       const int h = hb + u * RPW;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][0][i] = x[u][1][i] = 0.f;
-      if (h < h1) {
-        load8(src + static_cast<int64_t>(h) * HD + a0, x[u][0]);
-        load8(src + static_cast<int64_t>(h) * HD + b0, x[u][1]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int h = hb + u * RPW;
-      float (&a)[8] = x[u][0];
-      float (&b)[8] = x[u][1];
+      float a[8], b[8];
+      raw[u][0].widen(a);
+      raw[u][1].widen(b);
+      fetch(h + kAhead * RPW, raw[u]);
       if (h < p.n_q) {
         if (turns && turn_a) {                      // (a group that does not turn is left alone: infinity times a sine of zero would not be)
           if (p.interleaved) {
@@ -309,7 +327,7 @@ static int launch_store(const StoreParams& p, int num_sms, cudaStream_t stream) 
     // Rows of a warp: all of a token where there are tokens enough for eight warps an SM quarter, fewer (two steps at least) where there are not
     const int rpw = 512 / p.hd;
     int per = (rows + 2 * rpw - 1) / (2 * rpw) * (2 * rpw);
-    while (per > 2 * rpw && static_cast<int64_t>(p.T) * ((rows + per - 1) / per) < 32ll * num_sms) per = (per / 2 + 2 * rpw - 1) / (2 * rpw) * (2 * rpw);
+    while (per > 2 * rpw && static_cast<int64_t>(p.T) * ((rows + per - 1) / per) < 16ll * num_sms) per = (per / 2 + 2 * rpw - 1) / (2 * rpw) * (2 * rpw);
     const int64_t blocks = (static_cast<int64_t>(p.T) * ((rows + per - 1) / per) + 7) / 8;
     if (blocks > 0x7fffffff) return MB_ERR_TOO_LARGE;
     auto kern = p.hd == 64 ? store_rows_kernel<T, 64> : p.hd == 128 ? store_rows_kernel<T, 128> : store_rows_kernel<T, 256>;
