@@ -525,6 +525,7 @@ class PyDecoderExecutor {
     ex.final_norm = hold(final_norm);
     ex.lm_head = hold(lm_head);
     ex.cos_sin = static_cast<const float*>(hold(cos_sin));
+    ex.n_positions = static_cast<int>(cos_sin.size(0));
   }
   // scales: the four block-scale tensors of an fp8 layer (all or none)
   void add_layer(const Tensor& attn_norm, const Tensor& wqkv, const Tensor& wo,
@@ -573,6 +574,17 @@ class PyDecoderExecutor {
   // kv: [pages, 2, n_layers, n_kv, page_size, head_dim]
   void set_kv_cache(const Tensor& kv) {
     TORCH_CHECK(kv.dim() == 6 && kv.is_contiguous(), "kv cache must be 6-D contiguous");
+    // 8-bit rows: [pages, 2, layers, heads, page, head_dim + 1] bytes
+    ex.kv.fp8 = kv.scalar_type() == at::kByte;
+    ex.kv.pages = kv.size(0);
+    if (ex.kv.fp8) {
+      TORCH_CHECK(kv.size(5) == ex.cfg.head_dim + 1 && kv.size(4) % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.data_ptr()) & 15) == 0,
+                  "8-bit kv cache: [pages, 2, layers, heads, page, head_dim + 1] with pages of a multiple of 16 tokens");
+      const Tensor ws = torch::empty({static_cast<int64_t>(mb_paged_attention_fp8_workspace(1, 1, 1, 1, ex.cfg.n_q, ex.cfg.n_kv, ex.cfg.head_dim,
+                                                                                           ex.cfg.num_sms))}, kv.options());
+      ex.buf.kv8_ws = const_cast<void*>(hold(ws));
+      ex.buf.kv8_ws_bytes = ws.nbytes();
+    }
     ex.kv.base = const_cast<void*>(hold(kv));
     ex.kv.page_stride = kv.stride(0);
     ex.kv.kv_stride = kv.stride(1);

@@ -66,7 +66,8 @@ int mb_gemm_bf16_persistent(const void* X, const void* W, void* Y, const void* R
 // the norm and rope launches. `ssq` holds one sum of squares per row and 1024 columns, mb_ssq_blocks(hidden) of them.
 //   mb_gemm_bf16_partials: fp32 K splits of X · W^T in `ws` ([*splits][M][N]; MB_ERR_TOO_LARGE if one does not fit)
 //   mb_reduce_residual:    H += sum of splits, XW = H * (w + offset), ssq of H
-//   mb_reduce_rope_store:  QKV = sum of splits * factor, rotated, keys and values to the cache (ssq nullptr: factor 1)
+//   mb_reduce_rope_store:  QKV = sum of splits * factor, rotated, keys and values to the cache (ssq nullptr: factor 1); k_cache
+//                          nullptr: neither, QKV holds all rows as they are
 int mb_ssq_blocks(int hidden);
 int mb_gemm_bf16_partials(const void* X, const void* W, int M, int N, int K, int flags, void* ws, size_t ws_bytes,
                           int* splits, int* err, int num_sms, cudaStream_t stream);
@@ -603,6 +604,7 @@ typedef struct MbFp8Attention {
 } MbFp8Attention;
 size_t mb_paged_attention_fp8_workspace(int T, int B, int n_tiles, int n_decode, int n_q, int n_kv, int head_dim, int num_sms);
 int mb_paged_attention_fp8(const MbFp8Attention* a, const MbFp8Cache* cache, int num_sms, cudaStream_t stream);
+int mb_paged_attention_fp8_launches(const MbFp8Attention* a);      // kernels of that call
 
 #ifdef __cplusplus
 }

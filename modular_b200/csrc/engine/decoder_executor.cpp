@@ -68,6 +68,34 @@ bool DecoderExecutor::dec_usable(int T) const {
          mb_gemm_dec_plan(T, c.hidden, c.inter, 2, wsb, c.num_sms) == MB_OK;
 }
 
+int DecoderExecutor::attend_fp8(const StepInputs& in, int layer, cudaStream_t stream) {
+  const DecoderConfig& c = cfg;
+  const int qkv_dim = (c.n_q + 2 * c.n_kv) * c.head_dim, q_dim = c.n_q * c.head_dim;
+  char* base = static_cast<char*>(kv.base) + static_cast<int64_t>(layer) * kv.layer_stride;
+  const int64_t codes = static_cast<int64_t>(c.page_size) * c.head_dim;
+  MbFp8Cache cache = {};
+  cache.k = base; cache.v = base + kv.kv_stride;
+  cache.ks = reinterpret_cast<uint8_t*>(base + codes); cache.vs = reinterpret_cast<uint8_t*>(base + kv.kv_stride + codes);
+  cache.k_page = cache.v_page = cache.ks_page = cache.vs_page = kv.page_stride;
+  cache.k_head = cache.v_head = cache.ks_head = cache.vs_head = kv.head_stride;
+  cache.pages = kv.pages; cache.page_size = c.page_size;
+  MB_TRY(mb_rope_kv_store_fp8(buf.qkv, qkv_dim, buf.qkv, qkv_dim, 0, in.positions, in.slots, cos_sin, n_positions, &cache,
+                              in.T, c.n_q, c.n_kv, c.head_dim, c.head_dim, c.rope_interleaved, buf.err, c.num_sms, stream));
+  launches += 1;
+  mark("rope_kv_store", stream);
+  MbFp8Attention a = {};
+  a.q = buf.qkv; a.out = buf.attn;
+  a.block_table = in.block_table; a.q_start = in.q_start; a.q_len = in.q_len; a.kv_len = in.kv_len;
+  a.tile_seq = in.tile_seq; a.tile_q0 = in.tile_q0; a.decode_seq = in.decode_seq;
+  a.ws = buf.kv8_ws; a.ws_bytes = buf.kv8_ws_bytes; a.err = buf.err;
+  a.ldq = qkv_dim; a.ldo = q_dim; a.bt_stride = in.bt_stride; a.T = in.T; a.B = in.B;
+  a.n_tiles = in.n_tiles; a.n_decode = in.n_decode; a.n_q = c.n_q; a.n_kv = c.n_kv; a.head_dim = c.head_dim;
+  a.scale = c.attn_scale;
+  MB_TRY(mb_paged_attention_fp8(&a, &cache, c.num_sms, stream));
+  launches += mb_paged_attention_fp8_launches(&a);
+  return MB_OK;
+}
+
 int DecoderExecutor::forward_dec(const StepInputs& in, cudaStream_t stream) {
   const DecoderConfig& c = cfg;
   const int T = in.T;
@@ -101,7 +129,7 @@ int DecoderExecutor::forward_dec(const StepInputs& in, cudaStream_t stream) {
     char* kbase = static_cast<char*>(kv.base) + 2 * (static_cast<int64_t>(l) * kv.layer_stride);
     // one launch for the projection, the rotation and the cache store where the kernel takes the shape
     int fused = MB_ERR_SHAPE;
-    if (!c.rope_interleaved && w.wqkv_s == nullptr && w.qkv_bias == nullptr && w.q_norm == nullptr)
+    if (!kv.fp8 && !c.rope_interleaved && w.wqkv_s == nullptr && w.qkv_bias == nullptr && w.q_norm == nullptr)
       fused = mb_gemm_dec_qkv_rope(buf.xn, w.wqkv, T, c.hidden, c.hidden, c.hidden, buf.qkv, qkv_dim, in.positions,
                                    in.slots, cos_sin, kbase, kbase + 2 * kv.kv_stride, c.n_q, c.n_kv, c.head_dim,
                                    c.page_size, kv.page_stride, kv.head_stride, buf.dec_ws, buf.dec_ws_bytes,
@@ -122,13 +150,17 @@ int DecoderExecutor::forward_dec(const StepInputs& in, cudaStream_t stream) {
         launches += 1;
       }
       mark("gemm_qkv", stream);
-      MB_TRY(mb_rope_kv_store(buf.qkv, in.positions, in.slots, cos_sin, kbase, kbase + 2 * kv.kv_stride, T, c.n_q,
-                              c.n_kv, c.head_dim, c.page_size, kv.page_stride, kv.head_stride, c.rope_interleaved,
-                              stream));
-      launches += 1;
-      mark("rope_kv_store", stream);
+      if (!kv.fp8) {
+        MB_TRY(mb_rope_kv_store(buf.qkv, in.positions, in.slots, cos_sin, kbase, kbase + 2 * kv.kv_stride, T, c.n_q,
+                                c.n_kv, c.head_dim, c.page_size, kv.page_stride, kv.head_stride, c.rope_interleaved,
+                                stream));
+        launches += 1;
+        mark("rope_kv_store", stream);
+      }
     }
-    if (c.attn_impl == 1 && c.page_size % 64 == 0) {
+    if (kv.fp8) {
+      MB_TRY(attend_fp8(in, l, stream));
+    } else if (c.attn_impl == 1 && c.page_size % 64 == 0) {
       MB_TRY(mb_paged_attention_tma(
           buf.qkv, qkv_dim, buf.attn, q_dim, kv.base, kv.total_elems / hd,
           static_cast<long long>(l) * kv.layer_stride / hd,
@@ -141,7 +173,7 @@ int DecoderExecutor::forward_dec(const StepInputs& in, cudaStream_t stream) {
                                 in.n_decode, in.decode_seq, c.n_q, c.n_kv, c.head_dim, c.page_size, kv.page_stride,
                                 kv.head_stride, c.attn_scale, stream));
     }
-    launches += 1;
+    launches += kv.fp8 ? 0 : 1;
     mark("attention", stream);
     MB_TRY(dec(buf.attn, w.wo, w.wo_s, c.hidden, q_dim, 2, nullptr, 0, w.mlp_norm));
     mark("gemm_o+ar+norm", stream);
@@ -300,7 +332,7 @@ int DecoderExecutor::forward(const StepInputs& in, cudaStream_t stream) {
       MB_TRY(partials(buf.xn, w.wqkv, qkv_dim, c.hidden));
       mark("gemm_qkv", stream);
       MB_TRY(mb_reduce_rope_store(part, splits, l == 0 ? nullptr : ssq, c.hidden, c.eps, buf.qkv, in.positions,
-                                  in.slots, cos_sin, kc, vc, T, c.n_q, c.n_kv, c.head_dim, c.page_size,
+                                  in.slots, cos_sin, kv.fp8 ? nullptr : kc, kv.fp8 ? nullptr : vc, T, c.n_q, c.n_kv, c.head_dim, c.page_size,
                                   kv.page_stride, kv.head_stride, c.rope_interleaved, stream));
     } else if (w.wqkv_s != nullptr) {
       MB_TRY(linear_fp8(buf, c, buf.xn, c.hidden, w.wqkv, w.wqkv_s, buf.qkv, nullptr, T, qkv_dim, c.hidden,
@@ -316,15 +348,17 @@ int DecoderExecutor::forward(const StepInputs& in, cudaStream_t stream) {
       MB_TRY(mb_qk_norm(buf.qkv, w.q_norm, w.k_norm, T, c.n_q, c.n_kv, c.head_dim, qkv_dim, c.eps, stream));
       launches += 1;
     }
-    if (!lean) {
-      mark("gemm_qkv", stream);
+    if (!lean) mark("gemm_qkv", stream);
+    if (!lean && !kv.fp8) {
       MB_TRY(mb_rope_kv_store(buf.qkv, in.positions, in.slots, cos_sin, kc, vc, T, c.n_q, c.n_kv,
                               c.head_dim, c.page_size, kv.page_stride, kv.head_stride,
                               c.rope_interleaved, stream));
       launches += 1;
     }
     mark("rope_kv_store", stream);
-    if (c.attn_impl == 1 && c.page_size % 64 == 0) {
+    if (kv.fp8) {
+      MB_TRY(attend_fp8(in, l, stream));
+    } else if (c.attn_impl == 1 && c.page_size % 64 == 0) {
       const long long hd = c.head_dim;
       MB_TRY(mb_paged_attention_tma_step(
           buf.qkv, qkv_dim, buf.attn, q_dim, kv.base, kv.total_elems / hd,
@@ -527,11 +561,14 @@ int DecoderExecutor::forward_tp(const StepInputs& in, cudaStream_t stream) {
     }
     mark("gemm_qkv", stream);
     char* kbase = static_cast<char*>(kv.base) + 2 * (static_cast<int64_t>(l) * kv.layer_stride);
-    MB_TRY(mb_rope_kv_store(buf.qkv, in.positions, in.slots, cos_sin, kbase, kbase + 2 * kv.kv_stride, T,
-                            c.n_q, c.n_kv, c.head_dim, c.page_size, kv.page_stride, kv.head_stride,
-                            c.rope_interleaved, stream));
+    if (!kv.fp8)
+      MB_TRY(mb_rope_kv_store(buf.qkv, in.positions, in.slots, cos_sin, kbase, kbase + 2 * kv.kv_stride, T,
+                              c.n_q, c.n_kv, c.head_dim, c.page_size, kv.page_stride, kv.head_stride,
+                              c.rope_interleaved, stream));
     mark("rope_kv_store", stream);
-    if (c.attn_impl == 1 && c.page_size % 64 == 0) {
+    if (kv.fp8) {
+      MB_TRY(attend_fp8(in, l, stream));
+    } else if (c.attn_impl == 1 && c.page_size % 64 == 0) {
       MB_TRY(mb_paged_attention_tma(
           buf.qkv, qkv_dim, buf.attn, q_dim, kv.base, kv.total_elems / hd,
           static_cast<long long>(l) * kv.layer_stride / hd,
@@ -546,7 +583,7 @@ int DecoderExecutor::forward_tp(const StepInputs& in, cudaStream_t stream) {
                                 c.n_kv, c.head_dim, c.page_size, kv.page_stride, kv.head_stride,
                                 c.attn_scale, stream));
     }
-    launches += 2;
+    launches += kv.fp8 ? 0 : 2;
     mark("attention", stream);
     const void* next_norm = l + 1 < c.n_layers ? layers[l + 1].attn_norm : final_norm;
     MB_TRY(row_parallel_reduce_norm(buf.attn, w.wo, w.wo_s, q_dim, w.mlp_norm, false));

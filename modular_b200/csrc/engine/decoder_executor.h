@@ -74,6 +74,8 @@ struct DecoderBuffers {
   void* dec_ws = nullptr;       // decode-step GEMM partial tiles
   size_t dec_ws_bytes = 0;
   int* dec_state = nullptr;     // decode-step GEMM counters / all-reduce generation (zeroed once)
+  void* kv8_ws = nullptr;       // partial results of attention over an 8-bit cache
+  size_t kv8_ws_bytes = 0;
 };
 
 struct KVCacheView {
@@ -83,6 +85,8 @@ struct KVCacheView {
   int64_t layer_stride;  // elements between layers inside a page
   int64_t head_stride;   // elements between KV heads (= page_size * head_dim)
   int64_t total_elems;   // elements in the whole allocation
+  bool fp8 = false;      // 8-bit rows (kv_fp8.cu): the strides are bytes, a head of a page is its codes, then its exponents
+  int pages = 0;
 };
 
 // Device-resident per-step metadata (one packed H2D copy per step).
@@ -142,6 +146,7 @@ class DecoderExecutor {
   const void* final_norm = nullptr;
   const void* lm_head = nullptr;
   const float* cos_sin = nullptr;
+  int n_positions = 0;    // rows of cos_sin
   std::vector<DecoderLayerWeights> layers;
   long launches = 0;  // kernels launched since construction (for accounting)
 
@@ -163,6 +168,8 @@ class DecoderExecutor {
   std::vector<std::tuple<std::string, int, double>> profile_ms();
 
  private:
+  // Rotation and store of a step's rows in an 8-bit cache, and attention over it.
+  int attend_fp8(const StepInputs& in, int layer, cudaStream_t stream);
   int forward_tp(const StepInputs& in, cudaStream_t stream);
   // Small steps (T <= cfg.dec_max_tokens), one GPU or tensor parallel: four decode-step GEMMs per layer,
   // the row-parallel ones fused with all-reduce + residual + RMSNorm; no other collective, no stand-alone

@@ -163,3 +163,8 @@ extern "C" int mb_paged_attention_fp8(const MbFp8Attention* in, const MbFp8Cache
   auto kern = a.dtype == 0 ? attn_rows_kernel<__nv_bfloat16> : a.dtype == 1 ? attn_rows_kernel<float> : attn_rows_kernel<__half>;
   return launch_k(kern, dim3(a.T, a.n_q), dim3(128), 0, stream, p) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
+
+extern "C" int mb_paged_attention_fp8_launches(const MbFp8Attention* a) {
+  if (a->T <= 0 || a->B <= 0) return 0;
+  return on_tensor_cores(*a) ? (a->n_decode > 0 ? 2 : 0) + (a->n_tiles > 0 ? 2 : 0) : 1;
+}

@@ -1124,7 +1124,9 @@ reduce_residual_kernel(const float* __restrict__ part, int splits, __nv_bfloat16
 }
 
 // A thread finishes four dims of the first half of a query or key head and the matching four of the second (rotate-half)
-// or eight neighbours (interleaved), or four dims of a value head; the rotation works on the unrounded product.
+// or eight neighbours (interleaved), or four dims of a value head; the rotation works on the unrounded product. STORE false: no
+// rotation, and keys and values stay in the row (a cache of another form takes them from there).
+template <bool STORE>
 __global__ void __launch_bounds__(128)
 reduce_rope_store_kernel(const float* __restrict__ part, int splits, const float* __restrict__ ssq, int ssq_blocks,
                          float inv_cols, float eps, __nv_bfloat16* __restrict__ qkv,
@@ -1137,7 +1139,7 @@ reduce_rope_store_kernel(const float* __restrict__ part, int splits, const float
   const int t = blockIdx.y;
   int w = blockIdx.x * blockDim.x + threadIdx.x;
   if (w >= n_rot + n_kv * per_v) return;   // not the whole block: its other threads wait and trigger
-  const int64_t slot = slots[t];
+  const int64_t slot = STORE ? slots[t] : -1;
   const int row = (n_q + 2 * n_kv) * head_dim;
   const size_t stride = static_cast<size_t>(T) * row;
   const float* src = part + static_cast<size_t>(t) * row;
@@ -1152,7 +1154,7 @@ reduce_rope_store_kernel(const float* __restrict__ part, int splits, const float
   const bool rot = w < n_rot;
   const int h = rot ? w / per_rot : (w - n_rot) / per_v, d = (rot ? w % per_rot : (w - n_rot) % per_v) * 4;
   float4 c = {}, s = {};
-  if (rot) {
+  if (STORE && rot) {
     const float* cs = cos_sin + static_cast<size_t>(positions[t]) * head_dim + d;
     c = make_float4(cs[0], cs[1], cs[2], cs[3]);
     s = make_float4(cs[half], cs[half + 1], cs[half + 2], cs[half + 3]);
@@ -1161,7 +1163,9 @@ reduce_rope_store_kernel(const float* __restrict__ part, int splits, const float
   pdl_trigger();
   if (!rot) {
     const float4 v = sum_splits(src + (n_q + n_kv + h) * head_dim + d, stride, splits);
-    if (slot >= 0)
+    if (!STORE)
+      *reinterpret_cast<uint2*>(qkv + static_cast<size_t>(t) * row + (n_q + n_kv + h) * head_dim + d) = pack4(v.x * f, v.y * f, v.z * f, v.w * f);
+    else if (slot >= 0)
       *reinterpret_cast<uint2*>(v_cache + at + h * head_stride + d) = pack4(v.x * f, v.y * f, v.z * f, v.w * f);
     return;
   }
@@ -1170,7 +1174,10 @@ reduce_rope_store_kernel(const float* __restrict__ part, int splits, const float
   a.x *= f; a.y *= f; a.z *= f; a.w *= f;
   b.x *= f; b.y *= f; b.z *= f; b.w *= f;
   uint2 lo, hi;
-  if (interleaved) {
+  if (!STORE) {
+    lo = pack4(a.x, a.y, a.z, a.w);
+    hi = pack4(b.x, b.y, b.z, b.w);
+  } else if (interleaved) {
     lo = pack4(a.x * c.x - a.y * s.x, a.y * c.x + a.x * s.x, a.z * c.y - a.w * s.y, a.w * c.y + a.z * s.y);
     hi = pack4(b.x * c.z - b.y * s.z, b.y * c.z + b.x * s.z, b.z * c.w - b.w * s.w, b.w * c.w + b.z * s.w);
   } else {
@@ -1178,7 +1185,7 @@ reduce_rope_store_kernel(const float* __restrict__ part, int splits, const float
     hi = pack4(b.x * c.x + a.x * s.x, b.y * c.y + a.y * s.y, b.z * c.z + a.z * s.z, b.w * c.w + a.w * s.w);
   }
   __nv_bfloat16* dst;
-  if (h < n_q) {
+  if (!STORE || h < n_q) {
     dst = qkv + static_cast<size_t>(t) * row + h * head_dim;
   } else {
     if (slot < 0) return;
@@ -1678,7 +1685,8 @@ extern "C" int mb_reduce_rope_store(const float* part, int splits, const float* 
   if (T <= 0) return MB_OK;
   if (head_dim % 16 || splits < 1 || splits > kMaxSplits || T > 65535) return MB_ERR_SHAPE;
   const int work = (n_q + n_kv) * (head_dim / 8) + n_kv * (head_dim / 4);
-  return launch_k(reduce_rope_store_kernel, dim3((work + 127) / 128, T), dim3(128), 0, stream, part, splits, ssq,
+  auto kern = k_cache ? reduce_rope_store_kernel<true> : reduce_rope_store_kernel<false>;
+  return launch_k(kern, dim3((work + 127) / 128, T), dim3(128), 0, stream, part, splits, ssq,
                   mb_ssq_blocks(hidden), 1.0f / static_cast<float>(hidden), eps, static_cast<__nv_bfloat16*>(qkv),
                   positions, slots, cos_sin, static_cast<__nv_bfloat16*>(k_cache),
                   static_cast<__nv_bfloat16*>(v_cache), T, n_q, n_kv, head_dim, page_size, page_stride, head_stride,

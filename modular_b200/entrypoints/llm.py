@@ -88,12 +88,14 @@ class LLM:
                  step_token_alignment: Optional[int] = None, weights_are_sharded: bool = False,
                  ep_size: int = 1, ep_rank: int = 0, ep_fp8_dispatch: bool = False, speculative=None,
                  draft_model_config=None, draft_weights=None, num_state_slots: Optional[int] = None,
-                 max_logit_rows: int = 0):
+                 max_logit_rows: int = 0, kv_cache_format: Optional[str] = None):
         """``speculative``: a :class:`pipelines.speculative.SpeculativeConfig`; decode steps of greedy requests
         then verify proposals (several tokens per step, same output as plain greedy decoding): n-gram look-ups in
         the request's own history, or with ``method="draft_model"`` the greedy continuation of a smaller model of
         the same vocabulary (``draft_model_config`` / ``draft_weights``; random weights when none are given),
         which gets its own paged cache and drafts for all requests of a step at once.
+        ``kv_cache_format``: ``"float8_e4m3fn"`` keeps keys and values as e4m3 codes with an exponent per row (half the bytes of bf16);
+        a draft model keeps its own cache in the activations' dtype.
         ``num_state_slots``: recurrent-state slots of families that keep some (default: one per request of a batch)."""
         from ..models import family_for
 
@@ -173,7 +175,7 @@ class LLM:
             d_model = dfam.model_class(draft_model_config, draft_weights, d_kv.kv, max_tokens=max_batch_input_tokens,
                                        max_seqs=max_batch_size, max_position=max_length, **d_extra)
             self.draft = (d_model, d_kv)
-        kvp = fam.kv_params(model_config, page_size, dtype, enable_prefix_caching)
+        kvp = fam.cache_params(model_config, page_size, dtype, enable_prefix_caching, kv_cache_format)
         if num_kv_pages is None:
             if on_gpu:
                 free, total = torch.cuda.mem_get_info(self.device)

@@ -13,6 +13,8 @@ Device layout of the cache tensor (one allocation):
 
     [num_pages, 2 (K,V), num_layers, n_kv_heads, page_size, head_dim]   (MHA/GQA)
     [num_pages, 1,       num_layers, 1,          page_size, kv_lora + rope]  (MLA latent)
+    [num_pages, 2 (K,V), num_layers, n_kv_heads, page_size, head_dim + 1]    (8-bit rows, bytes: a head of a page is its codes, then
+                                                                              its exponents)
 
 so a (page, plane, layer, head) slice is one contiguous ``page_size x head_dim`` tile that a
 bulk copy or a TMA box can fetch in one piece, and a whole page (all layers) is contiguous
@@ -81,8 +83,18 @@ class KVCacheParams:
     state_specs: tuple = ()
     # further rows per token in the same pages, of the cache's dtype: (name, planes, width)
     paged_specs: tuple = ()
+    # None: rows of `dtype`; "float8_e4m3fn": rows of head_dim e4m3 codes and an exponent byte (``ops.fp8_cache_views``)
+    kv_format: Optional[str] = None
 
     def __post_init__(self):
+        if self.kv_format is not None:
+            if self.kv_format != "float8_e4m3fn":
+                raise ValueError(f"unknown kv cache format {self.kv_format!r} (None or 'float8_e4m3fn')")
+            if self.is_mla or self.paged_specs:
+                raise ValueError("an 8-bit cache holds keys and values per head: latent and paged extra rows stay in 16 bits")
+            if self.page_size % 16 or self.head_dim % 16 or self.head_dim > 256:
+                raise ValueError("an 8-bit cache has pages and heads of multiples of 16, heads of 256 at most")
+            self.dtype = torch.uint8
         if self.state_specs and self.enable_prefix_caching:
             raise ValueError("a recurrent state cannot be restored by prefix: prefix caching must be off")
 
@@ -99,10 +111,15 @@ class KVCacheParams:
     def bytes_per_page(self) -> int:
         el = torch.empty(0, dtype=self.dtype).element_size()
         extra = sum(planes * width for _, planes, width in self.paged_specs)
-        return (self.kv_dim * self.n_layers * self.n_kv_heads * self.head_dim + extra) * self.page_size * el
+        return (self.kv_dim * self.n_layers * self.n_kv_heads * self.row_elements + extra) * self.page_size * el
+
+    @property
+    def row_elements(self) -> int:
+        """Elements of one token's key (or value) of one head."""
+        return self.head_dim + (self.kv_format is not None)
 
     def shape(self, num_pages: int) -> tuple:
-        return (num_pages, self.kv_dim, self.n_layers, self.n_kv_heads, self.page_size, self.head_dim)
+        return (num_pages, self.kv_dim, self.n_layers, self.n_kv_heads, self.page_size, self.row_elements)
 
     def compute_num_device_blocks(self, available_bytes: int, max_batch: int = 0,
                                   max_len: int = 0) -> int:
@@ -342,8 +359,29 @@ class PagedKVCacheManager:
         blocks = np.asarray(st.blocks, dtype=np.int64)
         return blocks[pos // self.page_size] * self.page_size + pos % self.page_size
 
+    def read_tokens(self, request_id: str, layer: int, n_tokens: int, dtype: torch.dtype = torch.bfloat16):
+        """Keys (rotated) and values of a request's first ``n_tokens`` tokens in one layer, copied out of its pages: two tensors
+        [n_tokens, kv heads, head_dim]; 8-bit rows as the values they stand for, in ``dtype``. For inspection, and for taking a request
+        to a cache of another format."""
+        if self.params.is_mla:
+            raise ValueError("a latent cache holds no keys and values per head")
+        blocks = self._req[request_id].blocks
+        if not 0 <= n_tokens <= len(blocks) * self.page_size:
+            raise ValueError(f"{n_tokens} tokens of {len(blocks)} pages")
+        table = torch.tensor([blocks or [0]], dtype=torch.int32, device=self.device)
+        if self.params.kv_format is not None:
+            from .. import ops
+            one = lambda n: torch.tensor([n], dtype=torch.int32, device=self.device)  # noqa: E731
+            return ops.kv_load_fp8(*ops.fp8_cache_views(self.kv, layer), table, one(0), one(n_tokens), n_tokens, dtype)
+        rows = self.kv[table[0].long()][:, :, layer].permute(1, 0, 3, 2, 4)
+        return tuple(r.reshape(-1, *r.shape[2:])[:n_tokens].to(dtype) for r in rows)
+
     def layer_views(self, layer: int):
-        """(k_cache, v_cache) views [pages, n_kv, page_size, head_dim] of one layer."""
+        """(k_cache, v_cache) views [pages, n_kv, page_size, head_dim] of one layer; for an 8-bit cache
+        ``ops.fp8_cache_views``."""
+        if self.params.kv_format is not None:
+            from .. import ops
+            return ops.fp8_cache_views(self.kv, layer)
         if self.params.is_mla:
             return self.kv[:, 0, layer], None
         return self.kv[:, 0, layer], self.kv[:, 1, layer]

@@ -7,7 +7,7 @@ model directory) and lib/arch_lookup.py:70.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Any, Callable
 
 import torch
@@ -23,6 +23,16 @@ class ModelFamily:
     activation_bytes: Callable  # (cfg, max_tokens, max_seqs) -> int
     supports_tp: bool = False
     supports_ep: bool = False       # expert parallelism: routed experts sharded, every rank serves its own requests
+    kv_formats: tuple = ()          # cache formats besides the activations' dtype
+
+    def cache_params(self, cfg, page_size, dtype, prefix_caching, kv_format=None):
+        """``kv_params`` with the rows in ``kv_format`` (None: the activations' dtype)."""
+        params = self.kv_params(cfg, page_size, dtype, prefix_caching)
+        if kv_format is None:
+            return params
+        if kv_format not in self.kv_formats:
+            raise ValueError(f"the {self.name} family keeps its cache in the activations' dtype (kv cache format {kv_format!r})")
+        return replace(params, kv_format=kv_format)
 
 
 def _llama_family() -> ModelFamily:
@@ -36,7 +46,7 @@ def _llama_family() -> ModelFamily:
         return (T * (3 * cfg.hidden_size + 2 * cfg.q_dim + 3 * cfg.intermediate_size) * 2
                 + B * cfg.vocab_size * 4 + (256 << 20))
 
-    return ModelFamily("llama", Llama3Config, Llama3Weights, Llama3Model, kv, act, supports_tp=True)
+    return ModelFamily("llama", Llama3Config, Llama3Weights, Llama3Model, kv, act, supports_tp=True, kv_formats=("float8_e4m3fn",))
 
 
 def _deepseek_family() -> ModelFamily:

@@ -1038,7 +1038,6 @@ class Llama3Model:
             return self._forward_hidden_olmo(tokens, positions, slots, block_table, q_start, q_len, kv_len, plan, kv)
         h = ops.embedding(tokens, self.w.embed)
         for li, l in enumerate(self.w.layers):
-            kc, vc = kv[:, 0, li], kv[:, 1, li]
             x = ops.rms_norm(h, l.attn_norm, c.rms_norm_eps)
             if l.is_fp8:
                 # block-scaled fp8 projections: activations quantised per token group in front of every GEMM
@@ -1046,10 +1045,8 @@ class Llama3Model:
                 if l.qkv_bias is not None:
                     qkv += l.qkv_bias
                 self._qk_norm(qkv, l)
-                ops.rope_kv_store(qkv, positions, slots, self.cos_sin, kc, vc, c.num_attention_heads,
-                                  c.num_key_value_heads, c.head_dim, False)
-                a = ops.paged_attention(qkv, kc, vc, block_table, q_start, q_len, kv_len, c.num_attention_heads,
-                                        c.num_key_value_heads, c.head_dim, self.scale, plan=plan)
+                self._store(qkv, positions, slots, self.cos_sin, kv, li)
+                a = self._attend(qkv, kv, li, block_table, q_start, q_len, kv_len, plan)
                 h = ops.linear_fp8(a, l.wo, l.wo_s, residual=h)
                 x = ops.rms_norm(h, l.mlp_norm, c.rms_norm_eps)
                 act = ops.silu_mul(ops.linear_fp8(x, l.wgu, l.wgu_s))
@@ -1059,11 +1056,8 @@ class Llama3Model:
             if l.qkv_bias is not None:
                 qkv += l.qkv_bias
             self._qk_norm(qkv, l)
-            ops.rope_kv_store(qkv, positions, slots, self.cos_sin, kc, vc, c.num_attention_heads,
-                              c.num_key_value_heads, c.head_dim, False)
-            a = ops.paged_attention(qkv, kc, vc, block_table, q_start, q_len, kv_len,
-                                    c.num_attention_heads, c.num_key_value_heads, c.head_dim,
-                                    self.scale, plan=plan)
+            self._store(qkv, positions, slots, self.cos_sin, kv, li)
+            a = self._attend(qkv, kv, li, block_table, q_start, q_len, kv_len, plan)
             h = ops.linear(a, l.wo, residual=h)
             x = ops.rms_norm(h, l.mlp_norm, c.rms_norm_eps)
             if l.moe is not None:
@@ -1075,6 +1069,22 @@ class Llama3Model:
                 act = ops.silu_mul(ops.linear(x, l.wgu))
             h = ops.linear(act, l.wd, residual=h)
         return h
+
+    def _store(self, qkv, positions, slots, cos_sin, kv, layer: int) -> None:
+        """Rotates queries and keys and writes keys and values to the cache, whose dtype says its format (uint8: 8-bit rows)."""
+        c = self.cfg
+        heads = (c.num_attention_heads, c.num_key_value_heads, c.head_dim, False)
+        if kv.dtype == torch.uint8:
+            ops.rope_kv_store_fp8(qkv, positions, slots, cos_sin, *ops.fp8_cache_views(kv, layer), *heads)
+        else:
+            ops.rope_kv_store(qkv, positions, slots, cos_sin, kv[:, 0, layer], kv[:, 1, layer], *heads)
+
+    def _attend(self, qkv, kv, layer: int, block_table, q_start, q_len, kv_len, plan) -> torch.Tensor:
+        c = self.cfg
+        heads = (c.num_attention_heads, c.num_key_value_heads, c.head_dim, self.scale)
+        if kv.dtype == torch.uint8:
+            return ops.paged_attention_fp8(qkv, *ops.fp8_cache_views(kv, layer), block_table, q_start, q_len, kv_len, *heads, plan=plan)
+        return ops.paged_attention(qkv, kv[:, 0, layer], kv[:, 1, layer], block_table, q_start, q_len, kv_len, *heads, plan=plan)
 
     def _norm(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
         """The model's norm: RMSNorm with weight ``w``, or (OLMo) a LayerNorm without parameters, computed in fp32."""
@@ -1091,16 +1101,13 @@ class Llama3Model:
         for li, l in enumerate(self.w.layers):
             if l.is_fp8 or l.moe is not None or l.qkv_bias is not None:
                 raise ValueError("the OLMo layer variants are implemented for dense bf16 / fp32 weights without bias")
-            kc, vc = kv[:, 0, li], kv[:, 1, li]
             x = h if c.norm_after else self._norm(h, l.attn_norm)
             qkv = ops.linear(x, l.wqkv)
             if c.clip_qkv:
                 qkv.clamp_(-c.clip_qkv, c.clip_qkv)
             self._qk_norm(qkv, l)
-            ops.rope_kv_store(qkv, positions, slots, self.cos_sin, kc, vc, c.num_attention_heads,
-                              c.num_key_value_heads, c.head_dim, False)
-            a = ops.paged_attention(qkv, kc, vc, block_table, q_start, q_len, kv_len, c.num_attention_heads,
-                                    c.num_key_value_heads, c.head_dim, self.scale, plan=plan)
+            self._store(qkv, positions, slots, self.cos_sin, kv, li)
+            a = self._attend(qkv, kv, li, block_table, q_start, q_len, kv_len, plan)
             if c.norm_after:
                 h = h + self._norm(ops.linear(a, l.wo), l.attn_norm)
                 x = h
@@ -1125,14 +1132,11 @@ class Llama3Model:
         for li, l in enumerate(self.w.layers):
             if l.is_fp8 or l.moe is not None or l.qkv_bias is not None:
                 raise ValueError("Gemma layers are implemented for dense bf16 / fp32 weights without bias")
-            kc, vc = kv[:, 0, li], kv[:, 1, li]
             cos_sin = self.cos_sin_local if (li in c.local_layers and self.cos_sin_local is not None) else self.cos_sin
             qkv = ops.linear(ops.rms_norm(h, l.attn_norm, c.rms_norm_eps), l.wqkv)
             self._qk_norm(qkv, l)
-            ops.rope_kv_store(qkv, positions, slots, cos_sin, kc, vc, c.num_attention_heads, c.num_key_value_heads,
-                              c.head_dim, False)
-            a = ops.paged_attention(qkv, kc, vc, block_table, q_start, q_len, kv_len, c.num_attention_heads,
-                                    c.num_key_value_heads, c.head_dim, self.scale, plan=plan)
+            self._store(qkv, positions, slots, cos_sin, kv, li)
+            a = self._attend(qkv, kv, li, block_table, q_start, q_len, kv_len, plan)
             h = h + ops.rms_norm(ops.linear(a, l.wo), l.attn_out_norm, c.rms_norm_eps)
             gu = ops.linear(ops.rms_norm(h, l.mlp_norm, c.rms_norm_eps), l.wgu)
             act = torch.nn.functional.gelu(gu[:, :I], approximate="tanh") * gu[:, I:]
@@ -1168,7 +1172,6 @@ class Llama3Model:
 
         h = ops.embedding(tokens, self.w.embed)
         for li, l in enumerate(self.w.layers):
-            kc, vc = kv[:, 0, li], kv[:, 1, li]
             x = ops.rms_norm(h, l.attn_norm, c.rms_norm_eps)
             qkv = ops.linear(x, l.wqkv)
             if l.qkv_bias is not None:
@@ -1177,10 +1180,8 @@ class Llama3Model:
             add(qkv, lora.delta(li, "q_proj", x), 0, c.q_dim)
             add(qkv, lora.delta(li, "k_proj", x), c.q_dim, c.q_dim + c.kv_dim)
             add(qkv, lora.delta(li, "v_proj", x), c.q_dim + c.kv_dim, c.q_dim + 2 * c.kv_dim)
-            ops.rope_kv_store(qkv, positions, slots, self.cos_sin, kc, vc, c.num_attention_heads,
-                              c.num_key_value_heads, c.head_dim, False)
-            a = ops.paged_attention(qkv, kc, vc, block_table, q_start, q_len, kv_len, c.num_attention_heads,
-                                    c.num_key_value_heads, c.head_dim, self.scale, plan=plan)
+            self._store(qkv, positions, slots, self.cos_sin, kv, li)
+            a = self._attend(qkv, kv, li, block_table, q_start, q_len, kv_len, plan)
             h = add(ops.linear(a, l.wo, residual=h), lora.delta(li, "o_proj", a))
             x = ops.rms_norm(h, l.mlp_norm, c.rms_norm_eps)
             gu = ops.linear(x, l.wgu)

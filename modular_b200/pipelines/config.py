@@ -85,6 +85,8 @@ class KVCacheConfig(ConfigFileModel):
             raise ValueError("only the paged KV cache strategy exists")
         if self.kv_cache_page_size < 16 or self.kv_cache_page_size % 16:
             raise ValueError("kv_cache_page_size must be a positive multiple of 16")
+        if self.kv_cache_format not in (None, "float8_e4m3fn"):
+            raise ValueError("kv_cache_format is None (the model's dtype) or 'float8_e4m3fn'")
         if not (0.0 < self.device_memory_utilization <= 1.0):
             raise ValueError("device_memory_utilization must be in (0, 1]")
         return self

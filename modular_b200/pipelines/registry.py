@@ -93,7 +93,7 @@ class PipelineRegistry:
 
         dtype_bytes = 2
         fam = family_for(cfg)
-        kvp = fam.kv_params(cfg, pc.model.kv_cache.kv_cache_page_size, torch.bfloat16, True)
+        kvp = fam.cache_params(cfg, pc.model.kv_cache.kv_cache_page_size, torch.bfloat16, True, pc.model.kv_cache.kv_cache_format)
         free, total = torch.cuda.mem_get_info(device)
         act = fam.activation_bytes(cfg, pc.runtime.max_batch_input_tokens, pc.runtime.max_batch_size or 256)
         return MemoryEstimator.plan_from_sizes(
@@ -191,7 +191,7 @@ class PipelineRegistry:
                   device_memory_utilization=m.kv_cache.device_memory_utilization,
                   num_kv_pages=None if on_gpu else max(64, max_bs * ((max_length + m.kv_cache.kv_cache_page_size - 1)
                                                                      // m.kv_cache.kv_cache_page_size) + 1),
-                  enable_prefix_caching=m.kv_cache.enable_prefix_caching,
+                  enable_prefix_caching=m.kv_cache.enable_prefix_caching, kv_cache_format=m.kv_cache.kv_cache_format,
                   enable_chunked_prefill=rt.enable_chunked_prefill,
                   enable_in_flight_batching=rt.enable_in_flight_batching,
                   enable_overlap_scheduler=rt.enable_overlap_scheduler,

@@ -1,0 +1,185 @@
+"""The 8-bit key/value cache through the engine: LLM(kv_cache_format="float8_e4m3fn"), prefix caching and tiers over its pages, the native
+executor, captured graphs, rows read back, and what refuses the format."""
+
+import dataclasses
+
+import numpy as np
+import pytest
+import torch
+
+from modular_b200 import ops
+from modular_b200.entrypoints.llm import LLM
+from modular_b200.kv_cache import KVCacheParams
+from modular_b200.models.llama3 import LayerWeights, Llama3Config, Llama3Weights
+from modular_b200.pipelines.context import SamplingParams
+
+gpu = pytest.mark.gpu
+FP8 = "float8_e4m3fn"
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error(request):
+    yield
+    if torch.cuda.is_available() and "gpu" in request.keywords:
+        torch.cuda.synchronize()
+        ops.check_device_error()
+
+
+def confident(cfg, seed=0):
+    """Random weights whose output head is the embedding rolled by a few rows: every token has one clear successor, so that greedy tokens do not hang
+    on roundings."""
+    w = Llama3Weights.random_init(cfg, "cpu", torch.float32, seed=seed, std=0.03)
+    embed = torch.randn(cfg.vocab_size, cfg.hidden_size, generator=torch.Generator().manual_seed(seed + 1))
+    layers = [LayerWeights(**{f.name: None if getattr(l, f.name) is None else getattr(l, f.name).bfloat16().float() if torch.is_tensor(getattr(l, f.name))
+                              else getattr(l, f.name) for f in dataclasses.fields(l)}) for l in w.layers]
+    return Llama3Weights(embed.bfloat16().float(), layers, w.final_norm.bfloat16().float(), embed.roll(7, 0).bfloat16().float())
+
+
+def converted(w, device, dtype):
+    mv = lambda t: t.to(device=device, dtype=dtype) if torch.is_tensor(t) else t  # noqa: E731
+    layers = [LayerWeights(**{f.name: mv(getattr(l, f.name)) for f in dataclasses.fields(l)}) for l in w.layers]
+    return Llama3Weights(mv(w.embed), layers, mv(w.final_norm), mv(w.lm_head))
+
+
+SMALL = Llama3Config(hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=16, vocab_size=96,
+                     max_position_embeddings=256)
+ARGS = dict(device="cpu", dtype=torch.float32, max_length=128, max_batch_size=4, max_batch_input_tokens=32, num_kv_pages=32, page_size=16)
+GREEDY = SamplingParams(temperature=0.0, max_new_tokens=8, ignore_eos=True)
+
+
+def tokens(llm, prompts, sp=GREEDY):
+    return [r.tokens for r in llm.generate(prompts, sp)]
+
+
+def test_cache_of_half_the_bytes_and_the_same_tokens():
+    w = confident(SMALL)
+    plain, eight = LLM(SMALL, w, **ARGS), LLM(SMALL, w, kv_cache_format=FP8, **ARGS)
+    assert eight.kv.kv.dtype == torch.uint8 and tuple(eight.kv.kv.shape) == (32, 2, 2, 2, 16, 17)
+    assert eight.kv.params.bytes_per_page * 16 * 4 == plain.kv.params.bytes_per_page * 17        # (fp32 rows here)
+    prompts = [np.arange(50) % 96, np.arange(3), (np.arange(33) * 5) % 96]                            # several chunks of 32 tokens
+    assert tokens(eight, prompts) == tokens(plain, prompts)
+
+
+def test_prefix_pages_and_tiers_hold_8_bit_rows():
+    w = confident(SMALL)
+    a = dict(ARGS, num_kv_pages=9, host_kvcache_swap_space_gb=0.001)
+    llm = LLM(SMALL, w, kv_cache_format=FP8, **a)
+    prompt = np.arange(70) % 96
+    first = tokens(llm, [prompt])
+    assert llm.kv.prefix_hit_tokens == 0
+    assert tokens(llm, [prompt]) == first and llm.kv.prefix_hit_tokens >= 48
+    tokens(llm, [(np.arange(100) * 3 + 1) % 96])                                                     # pushes the first prompt's pages out
+    hits = llm.kv.tier_hit_tokens
+    assert tokens(llm, [prompt]) == first and llm.kv.tier_hit_tokens > hits
+
+
+@pytest.mark.parametrize("fmt", [None, FP8])
+def test_rows_read_back(fmt):
+    w = confident(SMALL)
+    llm = LLM(SMALL, w, kv_cache_format=fmt, **ARGS)
+    rid = llm.add_request(np.arange(40) % 96, SamplingParams(temperature=0.0, max_new_tokens=20, ignore_eos=True))
+    while llm._records[rid].first_token is None:
+        llm.step()
+    k, v = llm.kv.read_tokens(rid, 1, 40, torch.float32)
+    assert k.shape == v.shape == (40, 2, 16)
+    if fmt is None:
+        kc, vc = llm.kv.layer_views(1)
+        page = llm.kv.blocks_of(rid)[2]
+        assert torch.equal(k[32:40], kc[page, :, :8].transpose(0, 1)) and torch.equal(v[32:40], vc[page, :, :8].transpose(0, 1))
+    else:
+        # the same rows as a 16/32-bit cache, each code within half a step (2^-4) of the value, or of the row's smallest one
+        other = LLM(SMALL, w, **ARGS)
+        r2 = other.add_request(np.arange(40) % 96, SamplingParams(temperature=0.0, max_new_tokens=20, ignore_eos=True))
+        while other._records[r2].first_token is None:
+            other.step()
+        for mine, theirs in zip(llm.kv.read_tokens(rid, 0, 40, torch.float32), other.kv.read_tokens(r2, 0, 40, torch.float32)):
+            step = theirs.abs().amax(-1, keepdim=True) * 2.0 ** -17
+            assert ((mine - theirs).abs() <= 2.0 ** -4 * theirs.abs() + step + 1e-6).all()
+    with pytest.raises(ValueError):
+        llm.kv.read_tokens(rid, 0, 10_000)
+
+
+def test_what_refuses_the_format():
+    from modular_b200.models.deepseek_v3 import DeepseekV3Config
+    from modular_b200.pipelines.config import KVCacheConfig
+    w = confident(SMALL)
+    with pytest.raises(ValueError, match="format"):
+        LLM(SMALL, w, kv_cache_format="float8_e5m2", **ARGS)
+    with pytest.raises(ValueError):
+        KVCacheParams(2, 2, 16, 24, kv_format=FP8)
+    with pytest.raises(ValueError):
+        KVCacheParams(2, 2, 40, 16, kv_format=FP8)
+    with pytest.raises(ValueError):
+        KVCacheParams(2, 1, 576, 128, is_mla=True, kv_format=FP8)
+    with pytest.raises(ValueError):
+        KVCacheParams(2, 2, 16, 16, kv_format=FP8, paged_specs=(("rows", 1, 8),))
+    with pytest.raises(ValueError):
+        KVCacheConfig(kv_cache_format="int4")
+    assert KVCacheConfig(kv_cache_format=FP8).kv_cache_format == FP8
+    from modular_b200.models import family_for
+    fam = family_for(DeepseekV3Config())
+    with pytest.raises(ValueError, match="family"):
+        fam.cache_params(DeepseekV3Config(), 128, torch.bfloat16, False, FP8)
+
+
+# ------------------------------------------------------------------------------------------------------------ on a GPU
+MID = dict(hidden_size=512, intermediate_size=1024, num_hidden_layers=2, vocab_size=1024, max_position_embeddings=2048)
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(8, 2, 64, 128), (4, 4, 128, 64), (14, 2, 64, 16), (4, 1, 128, 128), (2, 2, 256, 32)])
+@pytest.mark.parametrize("executor", [True, False])
+def test_generation_matches_the_cpu_model_over_the_same_cache_format(heads, kv_heads, hd, page, executor):
+    """Ragged prompts in chunks, then decode steps (a captured graph among them), against fp32 on the CPU."""
+    cfg = Llama3Config(num_attention_heads=heads, num_key_value_heads=kv_heads, head_dim=hd, **MID)
+    w = confident(cfg, seed=hd + heads)
+    args = dict(max_length=1024, max_batch_size=8, max_batch_input_tokens=256, num_kv_pages=8192 // page, page_size=page, kv_cache_format=FP8)
+    prompts = [(np.arange(n) * 13 + n) % cfg.vocab_size for n in (300, 5, 64, 1, 129)]
+    want = tokens(LLM(cfg, w, device="cpu", dtype=torch.float32, **args), prompts)
+    llm = LLM(cfg, converted(w, "cuda", torch.bfloat16), device="cuda", dtype=torch.bfloat16, graph_batch_sizes=[5], **args)
+    assert llm.model.use_executor
+    if not executor:
+        llm = LLM(cfg, converted(w, "cuda", torch.bfloat16), device="cuda", dtype=torch.bfloat16, device_graph_capture=False,
+                  enable_overlap_scheduler=False, **args)
+        llm.model.use_executor = False
+        llm.pipeline.model.use_executor = False
+    assert tokens(llm, prompts) == want
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_executor_step_equals_the_same_step_op_by_op(T):
+    """One layer step of T tokens through the executor (small ones with the norms in the split-K reductions) and through the operators: logits within the
+    roundings of bf16 activations (2^-8 each, some ten in a row, on values of the logits' size)."""
+    cfg = Llama3Config(num_attention_heads=8, num_key_value_heads=2, head_dim=128, **MID)
+    w = converted(confident(cfg), "cuda", torch.bfloat16)
+    args = dict(device="cuda", dtype=torch.bfloat16, max_length=1024, max_batch_size=8, max_batch_input_tokens=256, num_kv_pages=64, kv_cache_format=FP8,
+                device_graph_capture=False)
+    llm = LLM(cfg, w, **args)
+    m = llm.model
+    tok = (torch.arange(T, device="cuda") * 7 + 3) % cfg.vocab_size
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.arange(1, 9, dtype=torch.int32, device="cuda").view(1, -1)
+    pos = torch.arange(T, device="cuda")
+    slots = table[0].long()[pos // 128] * 128 + pos % 128
+    want = m.forward_tensors(tok, pos.int(), slots, table, i32(0), i32(T), i32(T), torch.tensor([T - 1], device="cuda"))
+    rows = m.kv.clone()
+    m.kv.zero_()
+    rec = llm.generate([tok.cpu().numpy()], SamplingParams(temperature=0.0, max_new_tokens=1, ignore_eos=True))
+    assert rec[0].tokens == [int(want[0].argmax())]
+    got = m.logits_buf[0].float()
+    assert (got - want[0]).norm() <= 10 * 2.0 ** -8 * want[0].norm()
+    assert rows.any() and m.kv.any()
+
+
+@gpu
+def test_drafted_tokens_are_verified_over_the_format():
+    from modular_b200.pipelines.speculative import SpeculativeConfig
+    cfg = Llama3Config(num_attention_heads=8, num_key_value_heads=2, head_dim=64, **MID)
+    w = confident(cfg)
+    args = dict(max_length=512, max_batch_size=4, max_batch_input_tokens=256, num_kv_pages=64, kv_cache_format=FP8)
+    prompts = [(np.arange(n) * 5) % cfg.vocab_size for n in (70, 9)]
+    want = tokens(LLM(cfg, w, device="cpu", dtype=torch.float32, **args), prompts)
+    gw = converted(w, "cuda", torch.bfloat16)
+    spec = LLM(cfg, gw, device="cuda", dtype=torch.bfloat16, speculative=SpeculativeConfig("ngram", 3), **args)
+    assert tokens(spec, prompts) == want
