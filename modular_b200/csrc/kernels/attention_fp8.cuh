@@ -116,6 +116,10 @@ __device__ __forceinline__ void store4(__half* p, float4 v, float f) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_f16(v.x * f, v.y * f), pack_f16(v.z * f, v.w * f));
 }
 
+// bit 7 of each byte that is a NaN code (and others beside it)
+__device__ __forceinline__ uint32_t nan_sums(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return nan_sums(w) & 0x80808080u; }
+
 // attention_fp8_decode.cu: the sequences of the decode list; attention_fp8_chunk.cu: the tiles. 16-bit queries, heads of 64 or 128.
 size_t decode_workspace(int n_decode, int n_q, int n_kv, int head_dim, int num_sms);
 int decode_attention(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cudaStream_t stream);

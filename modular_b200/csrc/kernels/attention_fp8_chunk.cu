@@ -7,7 +7,9 @@
 //   warp 2        walks over the share and hands its pieces to the others
 //   warp 0        producer: codes and exponents of 64 tokens (bulk copies, the rows of a page and head lie together) into a ring
 //   warps 12-15   codes to f16, into operand tiles with the 128-byte swizzle. Within a tile a row's scale is applied relative to the largest
-//                 of the tile (a power of two: exact unless it is 2^-20 of that), so the tile has one scale left over, for K and for V
+//                 of the tile (a power of two: exact unless it is 2^-21 of that), so the tile has one scale left over, for K and for V.
+//                 A tile that holds keys some rows do not see is looked through: where a NaN among its values or a row's larger scale would reach rows
+//                 that must not see it, the tile is marked: it counts as hidden, and the softmax warps add its keys one by one to the finished sums
 //   warps 1, 3    MMA issuers, one per query tile: S_g = Q_g . K^T of the next keys into the other of two buffers, then O_g += P_g . V (P from TMEM)
 //   warps 4-11    softmax, a query row per thread (as attention_tc.cu). The tile's scale of K is part of the score's factor; that of V, 2^E, goes
 //                 into the exponent, 2^(t + E - m), and the denominator adds the tile's sum times 2^-E. The next segment's queries are brought in
@@ -45,8 +47,11 @@ struct ChunkParams {
   int box;
 };
 
+constexpr int kExact = 21;              // a scale so many powers of two under its tile's largest leaves f16 all bits of a code
+
 struct TileInfo {
   float k, v;                           // factor of a score, exponent of the values
+  uint8_t marked[4];                    // by either half of its keys, and of its values
 };
 // Tiles [ta, tb) of a segment's nt, as warp 2 hands them out
 struct Piece {
@@ -70,6 +75,8 @@ struct ChunkBars {
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
   TileInfo info[4];
+  uint8_t marked[2 * kPieces][4];       // marked tiles of a piece, by converter: bit 0 is the first tile that some row does not see all of
+  int3 marked_of[2 * kPieces];          // (if there are any) that tile, the piece's sequence and its kv_hi
   int rows[kRing];                      // keys of a tile
   int warp_sum[kThreads / 32];
   uint32_t tmem_base;
@@ -175,6 +182,84 @@ struct Pieces {
   }
 };
 
+// The keys of a marked tile, 32 at a time, added to a row's sums: O in TMEM, m and l. Every thread of the warp has a row; those that are not there see
+// nothing. x = t + e of a key waits in `turn`.
+template <int HD, typename T>
+__device__ __noinline__ float2 tile_by_hand(const ChunkParams& p, int seq, int head, const T* q, int kv0, int kv_hi, int limit, float2 ml, bool unset,
+                                            uint8_t* turn, uint32_t o_addr) {
+  const MbFp8Cache& c = p.c;
+  const int lane = threadIdx.x & 31;
+  const float sc = p.a.scale * kLog2e;
+  float m = ml.x, l = ml.y;
+  float* x = reinterpret_cast<float*>(turn) + lane;
+  auto place = [&](int key, const uint8_t*& codes, const uint8_t*& byte, bool is_v) {
+    const int nth = key / c.page_size, off = key - nth * c.page_size;
+    int page = nth < p.a.bt_stride ? p.a.block_table[static_cast<int64_t>(seq) * p.a.bt_stride + nth] : 0;
+    if (page < 0 || page >= c.pages) page = 0;      // (reported; some page stands in for it)
+    codes = static_cast<const uint8_t*>(is_v ? c.v : c.k) + page * (is_v ? c.v_page : c.k_page) + head * (is_v ? c.v_head : c.k_head) + static_cast<int64_t>(off) * HD;
+    byte = (is_v ? c.vs + page * c.vs_page + head * c.vs_head : c.ks + page * c.ks_page + head * c.ks_head) + off;
+  };
+  const int hi = min(kv0 + 64, kv_hi);
+#pragma unroll 1
+  for (int k0 = kv0; k0 < hi; k0 += 32) {
+    const int n = min(32, hi - k0);
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const uint8_t *codes, *byte;
+      place(k0 + j, codes, byte, false);
+      float acc = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < HD; i += 8) {
+        float y[8];
+        widen8<T>(*reinterpret_cast<const uint4*>(q + i), y);
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + i);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 f = two_codes((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+          acc = fmaf(f.y, y[e + 1], fmaf(f.x, y[e], acc));
+        }
+      }
+      const float scale = pow2_byte(*byte) * sc;
+      place(k0 + j, codes, byte, true);
+      const float t = fmaf(acc, scale, static_cast<float>(min(max(*byte, kLeastByte), kMostByte) - 127));
+      x[j * 32] = t;
+      if (k0 + j <= limit) top = fmaxf(top, t);
+    }
+    const float mn = unset ? (top == -INFINITY ? 0.f : top) : fmaxf(m, top), factor = unset ? 0.f : exp2f(m - mn);
+    unset = unset && top == -INFINITY;
+    m = mn;
+    l *= factor;
+#pragma unroll 1
+    for (int h = 0; h < HD / 32; ++h) {
+      uint32_t o[32];
+      tmem_ld_32x32(o_addr + h * 32, o);
+      tc_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        const uint8_t *codes, *byte;
+        place(k0 + j, codes, byte, true);
+        const float w = exp2f(x[j * 32] - m + kShift);
+        const bool seen = k0 + j <= limit;
+        if (h == 0 && seen) l = fmaf(w, pow2f(127 - min(max(*byte, kLeastByte), kMostByte)), l);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 f = two_codes(*reinterpret_cast<const uint16_t*>(codes + h * 32 + i));
+          if (seen) {
+            o[i] = __float_as_uint(fmaf(w * (1 << kHeadroom), f.x, __uint_as_float(o[i])));
+            o[i + 1] = __float_as_uint(fmaf(w * (1 << kHeadroom), f.y, __uint_as_float(o[i + 1])));
+          }
+        }
+      }
+      tmem_st_32x32(o_addr + h * 32, o);
+      tc_wait_st();
+    }
+  }
+  return make_float2(unset ? kNoMax : m, l);
+}
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ ChunkParams p) {
   using Sh = Shape<HD>;
@@ -203,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       for (int g = 0; g < 2; ++g) { mbar_init(&bars->s_full[g][b], 1); mbar_init(&bars->p_full[g][b], 4); mbar_init(&bars->pv_done[g][b], 1); }
       mbar_init(&bars->q_full[b], 4); mbar_init(&bars->o_done[b], 1); mbar_init(&bars->o_free[b], 4);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&bars->info_full[i], 2);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars->info_full[i], 4);
     for (int i = 0; i < kPieces; ++i) { mbar_init(&bars->piece_full[i], 1); mbar_init(&bars->piece_empty[i], kRoles); }
     bars->abort_word = 0;
     fence_mbar_init();
@@ -371,9 +456,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         if (lane == 0) mbar_arrive(&bars->piece_empty[i % kPieces]);
         if (nt < 0) break;
         if (active) { wait(q_full, q_ph, 762); q_ph ^= 1; }
-        if (ok && nt > 0) scores(active);
-        for (int t = 0; t < nt && ok; ++t) {
+        // (one place that makes scores: the code of all roles is more than the instruction cache holds, and every copy shows)
+        for (int t = -1; t < nt && ok; ++t) {
           if (t + 1 < nt) scores(active);
+          if (t < 0) continue;
           wait(&bars->v_full[vb], v_ph, 753);
           if (active) {
             if (t == 0) { wait(o_free, o_ph, 763); o_ph ^= 1; }
@@ -422,9 +508,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       if (!ok) break;
       const Piece& q = bars->piece[i % kPieces];
       const int nt = q.nt < 0 ? -1 : q.tb - q.ta;
+      const int all_see = max(0, q.kl - q.ql + q.tq0 + 1 - q.ta * 64), ta = q.ta, seq = q.seq, kv_hi = q.kv_hi;     // all_see: of the piece's keys, the first that some row does not see
+      uint32_t marked = 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->piece_empty[i % kPieces]);
       if (nt < 0) break;
+      if (lane == 0) bars->marked[i % (2 * kPieces)][cw] = 0;
       for (int t = 0; t < nt; ++t, ++ct) {
         const int b = ct & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[s], ph, abort_word, p.a.err, 755));
@@ -432,6 +521,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         const int n = bars->rows[s];
         const uint8_t* sc = sScale + s * 128 + kv * 64;
         const uint8_t* from = sRing + s * Sh::kStage + kv * Sh::kCodes + row0 * HD + chunk * 16;
+        bool nan = false;
+        if (kv == 1 && (t + 1) * 64 > all_see) {     // NaN among the values of keys that some row does not see
+          uint32_t sums = 0;
+#pragma unroll 1
+          for (int it = max(0, all_see - t * 64 - (cw & 1) * 32) / kRowStep; it < kSteps; ++it) {
+            if ((cw & 1) * 32 + it * kRowStep >= n) break;
+            const uint4 w = *reinterpret_cast<const uint4*>(from + it * kRowStep * HD);
+            if (row0 + it * kRowStep < n) sums |= nan_sums(w.x) | nan_sums(w.y) | nan_sums(w.z) | nan_sums(w.w);
+          }
+          nan = __any_sync(0xffffffffu, (sums & 0x80808080u) != 0);
+        }
         // all loads first: the stores that follow could not be told from them
         uint4 code[kSteps];
         int byte[kSteps];
@@ -447,17 +547,41 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         if (lane == 0) mbar_arrive(&bars->empty[s]);           // this warp's part of the stage is in registers
         ok = __all_sync(0xffffffffu, mbar_wait(&empty16[b], ((ct >> 1) & 1) ^ 1, abort_word, p.a.err, 756));
         if (!ok) break;
-        // (the products of two tiles ago are through, so the softmax is done with what four tiles ago stood here)
-        if ((cw & 1) == 0 && lane == 0) {
-          if (kv == 0) bars->info[ct & 3].k = score_factor(p.a.scale * kLog2e, top - 127 - kHeadroom);
-          else bars->info[ct & 3].v = static_cast<float>(top - 127);
-          mbar_arrive(&bars->info_full[ct & 3]);
-        }
         uint8_t* to = tile16 + b * Sh::kTile16;
         if (n < 64) {                                // rows behind the last key become zeros
 #pragma unroll
           for (int it = 0; it < kSteps; ++it)
             if (row0 + it * kRowStep >= n) { code[it] = make_uint4(0, 0, 0, 0); byte[it] = 0; }
+        }
+        bool mark = false;
+        if ((t + 1) * 64 > all_see) {
+          const int low = static_cast<int>(__reduce_min_sync(0xffffffffu, min(2 * lane < n ? two_bytes & 255u : 255u, 2 * lane + 1 < n ? two_bytes >> 8 : 255u)));
+          if (nan || top - low > kExact) {
+            mark = nan;
+#pragma unroll
+            for (int it = 0; it < kSteps; ++it) {
+              mark |= top - byte[it] > kExact && ((code[it].x | code[it].y | code[it].z | code[it].w) & 0x7f7f7f7fu) != 0;      // (rows of zeros may lie as low as they like)
+              if (nan) code[it] = make_uint4(0, 0, 0, 0);
+            }
+            mark = __any_sync(0xffffffffu, mark);
+            if (mark) {
+              marked |= 1u << (t - (all_see >> 6));
+              if (lane == 0) {
+                bars->marked[i % (2 * kPieces)][cw] = static_cast<uint8_t>(marked);
+                bars->marked_of[i % (2 * kPieces)] = make_int3(ta + (all_see >> 6), seq, kv_hi);
+              }
+            }
+          }
+        }
+        // (the products of two tiles ago are through, so the softmax is done with what four tiles ago stood here)
+        if (lane == 0) {
+          TileInfo& info = bars->info[ct & 3];
+          info.marked[cw] = mark;
+          if ((cw & 1) == 0) {
+            if (kv == 0) info.k = score_factor(p.a.scale * kLog2e, top - 127 - kHeadroom);
+            else info.v = static_cast<float>(top - 127);
+          }
+          mbar_arrive(&bars->info_full[ct & 3]);
         }
 #pragma unroll
         for (int it = 0; it < kSteps; ++it) {
@@ -566,15 +690,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           if (!ok) break;
           const float kf = fminf(fmaxf(bars->info[(ct + t) & 3].k * my_back, 1.1754944e-38f), 8.5e37f), ev = bars->info[(ct + t) & 3].v;       // (never zero)
           tc_fence_after();
+          const int kv0 = (ta + t) * 64, seen_to = *reinterpret_cast<const uint32_t*>(bars->info[(ct + t) & 3].marked) ? -1 : limit;
           uint32_t sr[2][32];
           tmem_ld_32x32(s_addr, sr[0]);
           tmem_ld_32x32(s_addr + 32, sr[1]);
           tc_wait_ld();
-          const int kv0 = (ta + t) * 64;
-          if (kv0 + 63 > limit) {
+          if (kv0 + 63 > seen_to) {
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              if (kv0 + c > limit) sr[c >> 5][c & 31] = __float_as_uint(-INFINITY);
+              if (kv0 + c > seen_to) sr[c >> 5][c & 31] = __float_as_uint(-INFINITY);
           }
           float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -645,6 +769,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         if (!ok) break;
         ++done;
         tc_fence_after();
+        uint32_t marked = *reinterpret_cast<const uint32_t*>(bars->marked[(at - 1) % (2 * kPieces)]);
+        if (__builtin_expect(marked != 0, 0)) {
+          marked |= marked >> 16;
+          marked = (marked | marked >> 8) & 255u;
+          const int3 of = bars->marked_of[(at - 1) % (2 * kPieces)];
+          const T* q = static_cast<const T*>(p.a.q) + (my_row ? static_cast<int64_t>(row) * p.a.ldq + static_cast<int64_t>(head) * HD : 0);
+          for (int t = of.x; marked != 0; ++t, marked >>= 1) {
+            if (!(marked & 1u)) continue;
+            const float2 ml = tile_by_hand<HD, T>(p, of.y, head / G, q, t * 64, of.z, my_row ? limit : -1, make_float2(m, l), unset, sTurn + (warp - 4) * Sh::kTurn, o_addr);
+            unset = ml.x == kNoMax;
+            m = unset ? 0.f : ml.x;
+            l = ml.y;
+          }
+        }
       }
       const float f = (whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f) * (1.f / (1 << kHeadroom));
       // 32 columns at a time turn round in shared memory, so that eight lanes write a row together. A piece that begins its CTA's share goes to slot 0,

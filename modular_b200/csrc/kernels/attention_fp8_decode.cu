@@ -266,6 +266,44 @@ __device__ __forceinline__ void walk32(RowState<HD, NR>& st, const uint32_t (&qf
   }
 }
 
+// Tokens [from, to) of this warp's 32 are hidden from some of the rows: NaN codes among their values become zeros in shared memory, for nothing times NaN
+// is NaN, and columns of rows that do see them NaN.
+template <int HD, int NR>
+__device__ __forceinline__ void set_nan_apart(RowState<HD, NR>& st, uint32_t sV, int row0, int lane, int k0, int from, int to, const int (&limit)[NR][2]) {
+  bool changed = false;
+#pragma unroll 1
+  for (int tok = from; tok < to; ++tok) {
+    const int row = row0 + tok - k0;
+    const uint32_t at = sV + row * HD + lane * 4;
+    uint32_t w = 0;
+    if (lane < HD / 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+    const uint32_t bad = nan_codes(w);
+    if (!__any_sync(0xffffffffu, bad != 0)) continue;
+    changed = true;
+    if (bad != 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w & ~((bad >> 7) * 255u)) : "memory");
+#pragma unroll 1
+    for (int pos = 0; pos < HD; ++pos) {
+      if (!((__shfl_sync(0xffffffffu, bad, pos >> 2) >> (8 * (pos & 3))) & 0x80u)) continue;
+      const int chunk = (pos >> 4) ^ (HD == 128 ? row & 7 : (row >> 1) & 3), col = chunk * 16 + (pos & 15);
+      if ((col & 15) >> 1 != lane >> 2) continue;
+#pragma unroll
+      for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (c == chunk && tok <= limit[r][e]) {
+              if (col & 1) st.o[c][r][2 + e] = NAN;
+              else st.o[c][r][e] = NAN;
+            }
+    }
+  }
+  if (changed) {
+    __syncwarp();
+    fence_proxy_async_smem();                        // (the next copy into this stage comes behind these stores)
+  }
+}
+
 template <int HD, int NR, typename T>
 __global__ void __launch_bounds__(Team<NR>::kThreads, kDecCtas)
 decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ DecParams p) {
@@ -485,7 +523,11 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
           const uint32_t sK = smem_u32(smem + s * kStage), sV = sK + kCodes, sE = smem_u32(sScale + s * 128 + row0);
           // the last tokens of a sequence are masked row by row; before them every row sees all
           if (k0 + 32 <= w.kl - w.ql + 1) walk32<HD, NR, false>(st, qf, sK, sV, sE, sc, row0, lane, k0, w.kl, limit);
-          else if (k0 < w.kl) walk32<HD, NR, true>(st, qf, sK, sV, sE, sc, row0, lane, k0, w.kl, limit);
+          else if (k0 < w.kl) {
+            // (with one group of rows every sequence has a single token)
+            if (NR > 1 && w.ql > 1) set_nan_apart<HD, NR>(st, sV, row0, lane, k0, max(k0, w.kl - w.ql + 1), min(k0 + 32, w.kl), limit);
+            walk32<HD, NR, true>(st, qf, sK, sV, sE, sc, row0, lane, k0, w.kl, limit);
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.empty[s]);
         }

@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(256) load_kernel(const MbFp8Cache c, const int
   if (threadIdx.x < kLoadRows) {
     const int64_t row = row0 + threadIdx.x;
     int64_t codes = -1, byte = 0;
-    if (row < rows) {
+    if (row < rows && B > 0) {
       int lo = 0, hi = B - 1;                        // the last sequence that starts at or before the row
       while (lo < hi) {
         const int m = (lo + hi + 1) >> 1;
@@ -457,7 +457,6 @@ extern "C" int mb_kv_load_fp8(const MbFp8Cache* cache, const int32_t* block_tabl
   if (rows <= 0) return MB_OK;
   const int rc = check_cache(cache, n_kv, head_dim);
   if (rc != MB_OK) return rc;
-  if (B < 1) return MB_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return MB_ERR_ALIGN;
   const long long blocks = (rows + kLoadRows - 1) / kLoadRows;
   if (blocks > 0x7fffffff) return MB_ERR_TOO_LARGE;

@@ -326,7 +326,9 @@ def rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale,
     T = qkv.shape[0]
     x = qkv[:, : (n_q + 2 * n_kv) * head_dim].reshape(T, n_q + 2 * n_kv, head_dim).double()
     if rot_dims:
-        cs = cos_sin[positions.long()].double().unsqueeze(1)
+        if bool(((positions[:T] < 0) | (positions[:T] >= cos_sin.shape[0])).any()):
+            raise ValueError(f"a position out of [0, {cos_sin.shape[0]})")
+        cs = cos_sin[positions[:T].long()].double().unsqueeze(1)
         c, s = cs[..., : rot_dims // 2], cs[..., rot_dims // 2:]
         turn = x[:, : n_q + n_kv, :rot_dims]
         if interleaved:
@@ -335,8 +337,10 @@ def rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale,
         else:
             a, b = turn[..., : rot_dims // 2].clone(), turn[..., rot_dims // 2:].clone()
             turn[..., : rot_dims // 2], turn[..., rot_dims // 2:] = a * c - b * s, b * c + a * s
-    q_out[:T, : n_q * head_dim] = x[:, :n_q].reshape(T, -1).to(qkv.dtype)
+    q_out[:T, : n_q * head_dim] = x[:, :n_q].reshape(T, n_q * head_dim).to(qkv.dtype)
     page = k_cache.shape[2]
+    if bool((slots[:T] >= k_cache.shape[0] * page).any()):
+        raise ValueError(f"a slot past the {k_cache.shape[0] * page} of the cache")
     ok = slots[:T] >= 0
     pg, off = slots[:T][ok] // page, slots[:T][ok] % page
     for part, cache, scale in ((x[:, n_q: n_q + n_kv], k_cache, k_scale), (x[:, n_q + n_kv:], v_cache, v_scale)):
@@ -347,7 +351,10 @@ def rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale,
 
 def _fp8_rows_of(cache, scale, pages, n, dtype):
     """Rows [0, n) of a sequence: [n, heads, head_dim]."""
-    pages = pages[: -(-n // cache.shape[2])].long()
+    need = -(-n // cache.shape[2])
+    pages = pages[:need].long()
+    if len(pages) < need or bool(((pages < 0) | (pages >= cache.shape[0])).any()):
+        raise ValueError(f"{n} tokens on pages {pages.tolist()} of {cache.shape[0]}")
     v = dequant_fp8_rows(cache.view(torch.uint8)[pages].view(torch.float8_e4m3fn), scale[pages], dtype)
     return v.transpose(1, 2).reshape(-1, cache.shape[1], cache.shape[3])[:n]
 
@@ -358,7 +365,7 @@ def kv_load_fp8(k_cache, v_cache, k_scale, v_scale, block_table, kv_start, kv_le
         for s in range(block_table.shape[0]):
             a, n = int(kv_start[s]), int(kv_len[s])
             if n > 0:
-                out[a: a + n] = _fp8_rows_of(cache, scale, block_table[s], n, out.dtype)
+                out[a: min(a + n, rows)] = _fp8_rows_of(cache, scale, block_table[s], n, out.dtype)[: max(0, rows - a)]
 
 
 def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, q_start, q_len, kv_len, n_q, n_kv, head_dim, scale, out):
@@ -374,7 +381,10 @@ def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, q_st
             hidden = torch.arange(kl, device=q.device).unsqueeze(0) > torch.arange(kl - ql, kl, device=q.device).unsqueeze(1)
             w = torch.einsum("qhd,khd->hqk", qq, k).mul(scale).masked_fill(hidden, float("-inf"))
             w = torch.exp(w - w.amax(-1, keepdim=True).clamp_min(-1e30))
-            o = torch.einsum("hqk,khd->qhd", w, v) / w.sum(-1).t().unsqueeze(-1).clamp_min(1e-37)      # (rows without keys: zero)
+            bad = torch.isnan(v)                                                                       # (zero times NaN would reach rows that do not see it)
+            o = torch.einsum("hqk,khd->qhd", w, v.masked_fill(bad, 0)) / w.sum(-1).t().unsqueeze(-1).clamp_min(1e-37)      # (rows without keys: zero)
+            if bool(bad.any()):
+                o.masked_fill_(torch.einsum("qk,khd->qhd", (~hidden).float(), bad.float()) > 0, math.nan)
         out[qs: qs + ql, : n_q * head_dim] = o.reshape(ql, -1).to(out.dtype)
 
 

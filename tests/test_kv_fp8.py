@@ -99,20 +99,18 @@ def attention(q, k, v, table, q_start, q_len, kv_len, n_q, n_kv, d, scale):
         out[a: a + n] = 0
         pages = table[s].long()[: -(-total // k.shape[2])]
         ks, vs = (x[pages].transpose(1, 2).reshape(-1, n_kv, d)[:total] for x in (k, v))
-        for h in range(n_q):
-            g = h // (n_q // n_kv)
-            for t in range(n):
-                seen = max(0, kv_len[s] - n + t + 1)
-                if seen == 0:
-                    continue
-                row = q[a + t, h * d: (h + 1) * d].double()
-                w = (ks[:seen, g] @ row) * scale
-                p = torch.exp(w - w.max())
-                p = p / p.sum()
-                out[a + t, h] = p @ vs[:seen, g]
-                A[a + t, h] = p @ vs[:seen, g].abs()
-                S[a + t, h] = (ks[:seen, g].abs() @ row.abs()).max() * scale
-                big[a + t, h] = vs[:seen, g].abs().max()
+        assert not ks.isnan().any() and not vs.isnan().any()
+        ks, vs = (x.repeat_interleave(n_q // n_kv, 1).transpose(0, 1) for x in (ks, vs))          # [n_q, total, d]
+        first = max(0, n - total)                                                                 # rows before it see nothing
+        for t0 in range(first, n, 64):
+            rows = torch.arange(t0, min(n, t0 + 64))
+            x = q[a + rows, : n_q * d].double().view(-1, n_q, d).transpose(0, 1)                  # [n_q, rows, d]
+            unseen = torch.arange(total) > (total - n + rows).unsqueeze(1)
+            p = torch.softmax((x @ ks.transpose(1, 2) * scale).masked_fill(unseen, -math.inf), -1)
+            out[a + rows] = (p @ vs).transpose(0, 1)
+            A[a + rows] = (p @ vs.abs()).transpose(0, 1)
+            S[a + rows] = (x.abs() @ ks.abs().transpose(1, 2) * scale).masked_fill(unseen, 0).amax(-1).transpose(0, 1).unsqueeze(-1)
+            big[a + rows] = vs.abs().amax(-1).unsqueeze(1).expand(-1, len(rows), -1).masked_fill(unseen, 0).amax(-1).transpose(0, 1).unsqueeze(-1)
     return out, A, big, S
 
 
@@ -129,14 +127,14 @@ def ints(a, device):
     return torch.tensor(a, dtype=torch.int32, device=device)
 
 
-def case(new, before, n_q, n_kv, d, page, dtype, device, seed=0, stale_nan=False, ld_extra=0, tail_rows=0):
+def case(new, before, n_q, n_kv, d, page, dtype, device, seed=0, stale_nan=False, ld_extra=0, tail_rows=0, v_spread=2.0):
     g = torch.Generator().manual_seed(seed)
     total = [n + b for n, b in zip(new, before)]
     need = [max(0, -(-t // page)) for t in total]
     pages = sum(need) + 2
     cache = Cache(pages, n_kv, page, d, device)
     k = torch.randn(pages, n_kv, page, d, generator=g, dtype=torch.float64) * torch.exp2(torch.randn(n_kv, 1, d, generator=g).clamp(-2, 2).double())
-    v = torch.randn(pages, n_kv, page, d, generator=g, dtype=torch.float64) * torch.exp2(2 * torch.randn(pages, n_kv, page, 1, generator=g).double())
+    v = torch.randn(pages, n_kv, page, d, generator=g, dtype=torch.float64) * torch.exp2((v_spread * torch.randn(pages, n_kv, page, 1, generator=g).double()).clamp(-45, 45))
     order = torch.randperm(pages, generator=g).tolist()
     table = torch.full((len(new), max(need + [1])), order[-1], dtype=torch.int32)
     at = 0
@@ -320,6 +318,265 @@ def test_rows_without_keys_are_zero(d, device):
     assert (rows[:2] == 0).all() and (rows[4] == 0).all() and (rows[5: 5 + 33] == 0).all() and (rows[2:4] != 0).any()
 
 
+@pytest.mark.parametrize("device", devices())
+def test_two_sequences_may_share_pages(device):
+    """A common prefix: both read the same pages, each its own last one."""
+    c = case([1, 40, 1], [70, 45, 90], 4, 2, 64, 16, torch.bfloat16, device, seed=8)
+    c["table"][1, :4] = c["table"][0, :4]
+    c["table"][2, :3] = c["table"][0, :3]
+    check_attention(run_attention(c), oracle(c), c["dtype"], 64, 91)
+
+
+@pytest.mark.parametrize("device", devices())
+def test_a_call_without_tokens_or_sequences(device):
+    cache, qkv, cs = _args(device)
+    none = torch.zeros(0, dtype=torch.int32, device=device)
+    assert ops.rope_kv_store_fp8(qkv[:0], none, none.long(), cs, *cache.views, 4, 2, 64).shape == (0, 256)
+    assert ops.paged_attention_fp8(qkv[:0], *cache.views, ints([[0]], device), ints([0], device), ints([0], device), ints([5], device), 4, 2, 64,
+                                   0.1).shape == (0, 256)
+    out = torch.full((3, 256), 2.0, dtype=torch.bfloat16, device=device)
+    ops.paged_attention_fp8(qkv, *cache.views, none.view(0, 1), none, none, none, 4, 2, 64, 0.1, out=out)
+    assert (out == 2).all()
+    for x in ops.kv_load_fp8(*cache.views, none.view(0, 1), none, none, 5):
+        assert x.shape == (5, 2, 64) and (x == 0).all()
+    assert ops.kv_load_fp8(*cache.views, ints([[0]], device), ints([0], device), ints([0], device), 0)[0].shape == (0, 2, 64)
+
+
+def test_the_codes_of_a_row_do_not_depend_on_its_neighbours():
+    """Rows of one call against calls of one token each."""
+    cache, qkv, cs = _args("cpu", T=16)
+    qkv = torch.randn(qkv.shape, generator=torch.Generator().manual_seed(1)).to(qkv.dtype)
+    pos, slots = torch.arange(16, dtype=torch.int32) % 4, torch.arange(16)
+    other, _, _ = _args("cpu", T=16)
+    cs = torch.rand(cs.shape, generator=torch.Generator().manual_seed(2))
+    ops.rope_kv_store_fp8(qkv.clone(), pos, slots, cs, *cache.views, 4, 2, 64)
+    for t in range(16):
+        ops.rope_kv_store_fp8(qkv[t: t + 1].clone(), pos[t: t + 1], slots[t: t + 1], cs, *other.views, 4, 2, 64)
+    assert torch.equal(cache.kv, other.kv)
+
+
+# ------------------------------------------------------------------------------------------------------------ larger sizes, graphs, streams
+@gpu
+@pytest.mark.parametrize("T,n_q,n_kv,d,rot,interleaved", [(1, 32, 8, 128, 128, False), (130, 32, 8, 128, 128, True), (1201, 8, 2, 64, 32, False),
+                                                          (700, 64, 28, 128, 128, False), (2500, 4, 1, 256, 64, False), (333, 3, 5, 96, 48, True)])
+def test_store_of_many_tokens(T, n_q, n_kv, d, rot, interleaved):
+    """Enough tokens that a warp takes all rows of one, and few of many rows."""
+    page, n_pos = 16, 5000
+    g = torch.Generator().manual_seed(T)
+    cache = Cache(-(-T // page) + 3, n_kv, page, d, "cuda")
+    x = torch.randn(T, (n_q + 2 * n_kv) * d, generator=g).bfloat16()
+    pos = torch.randint(0, n_pos, (T,), generator=g).int()
+    ang = torch.rand(n_pos, rot // 2, generator=g) * 50
+    cs = torch.cat([ang.cos(), ang.sin()], 1)
+    slots = torch.randperm(cache.kv.shape[0] * page, generator=g)[:T]
+    q = ops.rope_kv_store_fp8(x.cuda(), pos.cuda(), slots.cuda(), cs.cuda(), *cache.views, n_q, n_kv, d, interleaved=interleaved, rot_dims=rot)
+    r = x.double().view(T, -1, d)
+    r = torch.cat([rotate(r[:, : n_q + n_kv], cs.double()[pos.long()], rot, interleaved), r[:, n_q + n_kv:]], 1)
+    want = r[:, :n_q].reshape(T, -1)
+    assert ((q.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -22 * x.double().abs().amax(1, keepdim=True)).all()
+    have = [v.cpu() for v in cache.views]
+    for i, part in enumerate((r[:, n_q: n_q + n_kv], r[:, n_q + n_kv:])):
+        codes, e = quantise(part)
+        assert torch.equal(have[2 + i][slots // page, :, slots % page], e)
+        assert torch.equal(have[i].float()[slots // page, :, slots % page].double(), codes)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n_q,n_kv,d,page,new,before", [
+    (4, 1, 128, 128, [1, 1, 1], [4095, 2, 1500]),                 # one head: a tile a block
+    (8, 8, 64, 16, [1] * 6, [3000, 17, 900, 0, 2047, 64]),        # shares that hold several sequences and pieces of others
+    (32, 8, 128, 128, [1] * 40, [37 * i for i in range(40)]),
+    (16, 1, 64, 64, [1, 1], [4000, 100]),                         # two groups of eight rows
+    (8, 2, 128, 48, [4, 2, 1, 3], [2000, 0, 777, 64]),            # several tokens of a sequence
+    (4, 1, 128, 128, [200, 130, 1], [3800, 0, 4000]),             # long chunks and a single token
+    (16, 2, 64, 16, [70, 300, 2], [3500, 1000, 1]),
+    (32, 8, 128, 32, [64], [4000]),
+    (64, 1, 128, 128, [33, 5], [1900, 3000]),                     # one head for 64
+    (12, 4, 128, 128, [65, 1, 129, 7] * 5, [63, 0, 1, 640] * 5),
+    (6, 2, 80, 16, [1, 30], [2000, 1500]),                        # a head width of the CUDA cores
+])
+def test_long_contexts_shared_out(n_q, n_kv, d, page, new, before, dtype):
+    c = case(new, before, n_q, n_kv, d, page, DTYPES[dtype], "cuda", seed=n_q + d, stale_nan=True)
+    got = run_attention(c)
+    check_attention(got, oracle(c), c["dtype"], d, c["n_keys"])
+    assert torch.equal(got, run_attention(c))                     # sums are taken in one order
+
+
+@gpu
+@pytest.mark.parametrize("new,before", [([1, 1], [700, 3000]), ([64, 200, 1], [1500, 0, 400])])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_of_very_different_magnitudes(new, before, d):
+    """Rows of values up to 2^90 apart: the weights carry their exponents. And rows of zeros among them."""
+    c = case(new, before, 8, 2, d, 64, torch.bfloat16, "cuda", seed=d, stale_nan=False, v_spread=18.0)
+    check_attention(run_attention(c), oracle(c), c["dtype"], d, c["n_keys"])
+    c = case(new, before, 8, 2, d, 64, torch.bfloat16, "cuda", seed=d, stale_nan=False)
+    zero = torch.rand(c["held"][1].shape[:3], generator=torch.Generator().manual_seed(4)) < 0.5
+    c["held"][1][zero] = 0
+    c["cache"].views[1].view(torch.uint8).masked_fill_(zero.cuda().unsqueeze(-1), 0)
+    c["cache"].views[3].masked_fill_(zero.cuda(), 27)
+    check_attention(run_attention(c), oracle(c), c["dtype"], d, c["n_keys"])
+
+
+@pytest.mark.parametrize("device", devices())
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("n_q,n_kv", [(4, 2), (16, 1), (3, 3)])
+@pytest.mark.parametrize("at", [(1, 40), (0, 3), (2, 69), (2, 68)])
+def test_nan_reaches_the_rows_that_see_it_and_no_other(at, n_q, n_kv, d, device):
+    """A NaN code among the values of one token and head (its column), then among its keys (its row): tokens of the same chunk before it see neither."""
+    new, before = [3, 70], [62, 100]
+    if device == "cpu":
+        new, before = [3, 70], [10, 5]
+    c = case(new, before, n_q, n_kv, d, 16, torch.bfloat16, device, seed=d + n_q)
+    key = [before[s] + min(t, new[s] - 1) for s, t in enumerate(at)]
+    col, kvh = 13, n_kv - 1
+    want = oracle(c)
+    G = n_q // n_kv
+    for plane in (1, 0):
+        cells = [(int(c["table"][s, k // 16]), kvh, k % 16) for s, k in enumerate(key)]
+        kept = []
+        for cell in cells:
+            row = c["cache"].views[plane].view(torch.uint8)[cell]
+            kept.append(row.clone())
+            row[col] = 0xFF
+            if plane == 1:
+                c["held"][1][cell][col] = 0
+        got = run_attention(c).cpu().view(-1, n_q, d)
+        if plane == 1:
+            want = oracle(c)
+        clean = [x.clone() for x in want]
+        for s, k in enumerate(key):
+            sees = slice(c["start"][s] + k - before[s], c["start"][s] + new[s])
+            hit = got[sees, kvh * G: (kvh + 1) * G]
+            hit = hit[..., col] if plane == 1 else hit
+            assert hit.numel() and hit.isnan().all()
+            (clean[0][sees, kvh * G: (kvh + 1) * G, col] if plane == 1 else clean[0][sees, kvh * G: (kvh + 1) * G]).fill_(math.nan)
+        assert torch.equal(got.isnan(), clean[0].isnan())
+        check_attention(got.reshape(-1, n_q * d), clean, c["dtype"], d, c["n_keys"])
+        for cell, row in zip(cells, kept):
+            c["cache"].views[plane].view(torch.uint8)[cell] = row
+
+
+@pytest.mark.parametrize("device", devices())
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_much_larger_rows_that_come_later(d, dtype, device):
+    """Keys and values 2^40 times as large further on in a chunk leave the rows before them what they are."""
+    new, before = [70, 5, 200], [30, 60, 1]
+    c = case(new, before, 4, 2, d, 16, DTYPES[dtype], device, seed=d)
+    want = oracle(c)
+    big = [33, 3, 130]
+    for s, t in enumerate(big):
+        for k in range(before[s] + t, before[s] + new[s], 2):
+            cell = (int(c["table"][s, k // 16]), slice(None), k % 16)
+            for i in (2, 3):
+                c["cache"].views[i][cell] += 40
+    got = run_attention(c).cpu()
+    for s, t in enumerate(big):
+        want[0][c["start"][s] + t: c["start"][s] + new[s]] = math.nan
+    check_attention(got, want, c["dtype"], d, c["n_keys"])
+
+
+@gpu
+@pytest.mark.parametrize("new", [[1] * 4200, [1, 2] * 2100, [210, 213] * 20])
+def test_more_sequences_and_tiles_than_a_launch_takes(new):
+    n_q, n_kv = (64, 1) if len(new) < 100 else (2, 1)
+    g = torch.Generator().manual_seed(6)
+    before = torch.randint(0, 40, (len(new),), generator=g).tolist()
+    c = case(new, before, n_q, n_kv, 64, 16, torch.bfloat16, "cuda", seed=1, stale_nan=True)
+    check_attention(run_attention(c), oracle(c), c["dtype"], 64, c["n_keys"])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_a_cache_of_more_than_four_gigabytes(dtype):
+    """Pages whose offsets pass 32 bits: stored to, read back, attended to by single tokens and by a chunk."""
+    n_q, n_kv, d, page, pages, layers = 4, 2, 128, 128, 700, 96
+    big = torch.empty(pages, 2, layers, n_kv, page, d + 1, dtype=torch.uint8, device="cuda")
+    assert big.numel() > 2 ** 32
+    views = ops.fp8_cache_views(big, layers - 1)
+    g = torch.Generator().manual_seed(2)
+    total, table = 300, torch.tensor([[699, 3, 698]], dtype=torch.int32)
+    t = torch.arange(total)
+    slots = table[0].long()[t // page] * page + t % page
+    x = torch.randn(total, (n_q + 2 * n_kv) * d, generator=g).to(DTYPES[dtype])
+    ops.rope_kv_store_fp8(x.cuda(), t.int().cuda(), slots.cuda(), None, *views, n_q, n_kv, d, rot_dims=0)
+    r, held = x.double().view(total, -1, d), []
+    for part in (r[:, n_q: n_q + n_kv], r[:, n_q + n_kv:]):
+        y, e = quantise(part)
+        y = y * 2.0 ** (e.double() - 127).unsqueeze(-1)
+        held.append(torch.cat([y, torch.zeros(3 * page - total, n_kv, d, dtype=torch.float64)]).view(3, page, n_kv, d).transpose(1, 2))
+    for got, want in zip(ops.kv_load_fp8(*views, table.cuda(), ints([0], "cuda"), ints([total], "cuda"), total, torch.float32), held):
+        assert torch.equal(got.cpu().double(), want.transpose(1, 2).reshape(-1, n_kv, d)[:total])
+    for n in (1, 150):
+        q = x[-n:, : n_q * d].contiguous()
+        got = ops.paged_attention_fp8(q.cuda(), *views, table.cuda(), ints([0], "cuda"), ints([n], "cuda"), ints([total], "cuda"), n_q, n_kv, d, 0.1)
+        check_attention(got, attention(q, *held, torch.arange(3).view(1, 3), [0], [n], [total], n_q, n_kv, d, 0.1), DTYPES[dtype], d, total)
+
+
+@gpu
+def test_captured_steps_and_calls_on_two_streams():
+    """Two captured steps of one plan replayed in turn with other lengths, pages and queries, and calls on a second stream: none shares a workspace."""
+    new, n_q, n_kv, d = [1, 1, 80, 1], 8, 2, 128
+    cs = [case(new, b, n_q, n_kv, d, 64, torch.bfloat16, "cuda", seed=20 + i) for i, b in enumerate(([900, 1500, 700, 40], [31, 2000, 0, 1100], [0, 5, 1999, 64]))]
+    width = max(c["table"].shape[1] for c in cs)
+    wide = [torch.nn.functional.pad(c["table"], (0, width - c["table"].shape[1])).cuda() for c in cs]
+    want = [oracle(c) for c in cs]
+    plan = tuple(torch.from_numpy(a).cuda() for a in ops.build_attention_plan(new, n_q, n_kv))
+    pages = max(c["cache"].kv.shape[0] for c in cs)
+    graphs = []
+    for _ in range(2):
+        kv = torch.zeros(pages, *cs[0]["cache"].kv.shape[1:], dtype=torch.uint8, device="cuda")
+        s = dict(kv=kv, q=torch.zeros_like(cs[0]["q"]), table=torch.zeros_like(wide[0]), total=ints([1, 1, 80, 1], "cuda"),
+                 start=ints(cs[0]["start"], "cuda"), new=ints(new, "cuda"))
+        s["run"] = lambda s=s: ops.paged_attention_fp8(s["q"], *ops.fp8_cache_views(s["kv"], 1), s["table"], s["start"], s["new"], s["total"], n_q, n_kv, d,
+                                                       cs[0]["scale"], plan=plan)
+        s["run"]()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            s["out"] = s["run"]()
+        s["graph"] = graph
+        graphs.append(s)
+
+    def put(s, i):
+        s["kv"][: cs[i]["cache"].kv.shape[0]].copy_(cs[i]["cache"].kv)
+        s["q"].copy_(cs[i]["q"])
+        s["table"].copy_(wide[i])
+        s["total"].copy_(ints(cs[i]["total"], "cuda"))
+
+    for i, j in ((0, 1), (1, 2), (2, 0)):
+        put(graphs[0], i)
+        put(graphs[1], j)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        for s, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                s["graph"].replay()
+        torch.cuda.synchronize()
+        outs = []
+        for k in range(6):
+            with torch.cuda.stream(streams[k % 2]):
+                outs.append(graphs[k % 2]["run"]())
+        torch.cuda.synchronize()
+        for s, w in ((graphs[0], i), (graphs[1], j)):
+            check_attention(s["out"], want[w], torch.bfloat16, d, cs[w]["n_keys"])
+        for k, out in enumerate(outs):
+            assert torch.equal(out, graphs[k % 2]["out"])
+
+
+@gpu
+@pytest.mark.parametrize("n_tok", [3, 20])
+def test_a_plan_of_other_sequences_is_reported(n_tok):
+    """A plan that calls a sequence of 3 tokens with 8 heads each a single row."""
+    c = case([n_tok], [50], 16, 2, 64, 16, torch.bfloat16, "cuda", seed=1)
+    run_attention(c, plan=(None, None, ints([0], "cuda")))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError):
+        ops.check_device_error()
+    check_attention(run_attention(c), oracle(c), c["dtype"], 64, c["n_keys"])
+
+
 def test_a_step_through_store_attention_and_load():
     """The operators together on the CPU, as a model's layer calls them: a prompt in two chunks, then single tokens."""
     _run_together("cpu", torch.float32)
@@ -419,6 +676,19 @@ def test_refusals_of_layout_and_device():
     with pytest.raises(RuntimeError):
         ops.paged_attention_fp8(qkv, k, v, ks, vs, ints([[0]], "cuda"), ints([0], "cuda"), ints([3], "cuda"), ints([], "cuda"), 4, 2, 64, 0.1,
                                 plan=(None, None, None))
+
+
+def test_pages_slots_and_positions_out_of_range_raise():
+    cache, qkv, cs = _args()
+    one = lambda *a: ints(a, "cpu")  # noqa: E731
+    for pos, slot in (([0, 9, 1], [0, 1, 2]), ([0, -1, 1], [0, 1, 2]), ([0, 1, 2], [0, 64, 2])):
+        with pytest.raises(ValueError):
+            ops.rope_kv_store_fp8(qkv, one(*pos), torch.tensor(slot), cs, *cache.views, 4, 2, 64)
+    for table, n in (([[99]], 5), ([[-3]], 5), ([[0]], 40)):
+        with pytest.raises(ValueError):
+            ops.paged_attention_fp8(qkv, *cache.views, ints(table, "cpu"), one(0), one(3), one(n), 4, 2, 64, 0.1)
+        with pytest.raises(ValueError):
+            ops.kv_load_fp8(*cache.views, ints(table, "cpu"), one(0), one(n), n)
 
 
 @gpu
