@@ -1,6 +1,8 @@
 // Attention of sequences of few rows (single tokens, up to 16 query rows per key/value head) over the 8-bit paged cache.
 //
-// What bounds it is reading the cache: 2 (HD + 1) bytes a token and head, and 24 codes a cycle and SM to unpack on the way.
+// What bounds it is reading the cache: 2 (HD + 1) bytes a token and head, and 24 codes a cycle and SM to unpack on the way. 192 sequences of 2031 tokens
+// on average, 32 over 8 heads of 128: 149 us, 5.4 TB/s (when it took 161, the same loads without the work took 151). Three sequences of 50000: 61 us, 5.1 TB/s. One of 331
+// tokens: 10 us, a chain of latencies: lengths, pages, tiles, the join of the pieces in a second launch.
 //
 //   * The 64-token tiles of all sequences are one line of work per head, cut into equal shares (two tiles at least) for as many CTAs
 //     as the SMs hold. A sequence inside one share is finished there; the pieces of one that is cut go to the workspace and

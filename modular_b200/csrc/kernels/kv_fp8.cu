@@ -137,7 +137,7 @@ __device__ __forceinline__ Place place_of(const MbFp8Cache& c, bool is_v, int64_
   return at;
 }
 
-// Any head width and any pairs: a row is held by LANES lanes of a warp (hd / 8 of them at work); rows of a token in turn: queries, keys, values.
+// Any head width and any pairs, one row at a time: for the widths and rotations that the next kernel does not take. A row is held by LANES lanes of a warp (hd / 8 of them at work); rows of a token in turn: queries, keys, values.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) store_kernel(const StoreParams p) {
   pdl_wait();
@@ -210,7 +210,10 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreParams p) {
 
 // Heads of 64, 128 or 256 whose pairs lie in whole groups of eight. HD / 16 lanes hold a row, each two groups of eight columns: the two halves of eight
 // pairs, or two neighbouring groups. A warp takes one token and walks over some of its rows, 32 / LANES at a time, with the angles in registers: they
-// are read once for all heads (a thread an element group with its own angles: 108 us for 8192 tokens of 32 + 2 x 8 heads of 128).
+// are read once for all heads. The next rows are on their way while a step's are worked on. 8192 tokens of 32 + 2 x 8 heads of 128: 45 us, 4.2 TB/s (a
+// thread an element group with its own angles: 108 us; rows fetched when they are needed: 65). What bounds it is not the memory but how much of it eight
+// warps an SM quarter keep on the way beside the exact rotation of keys; more blocks with fewer registers were slower. 64 tokens: 5 us, the latency of
+// position, angles and row one after the other.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) store_rows_kernel(const StoreParams p, int per_warp) {
   constexpr int LANES = HD / 16, RPW = 32 / LANES;
@@ -342,7 +345,8 @@ static int launch_store(const StoreParams& p, int num_sms, cudaStream_t stream) 
 
 // Rows [0, kv_len[s]) of every sequence at kv_start[s] of the outputs; rows that belong to no sequence are zeros. A block takes 64 rows of all heads,
 // keys or values by grid.y: it looks each row's place up once, then eight codes a thread, a head at a time (the tokens of a page and head lie
-// together). Sixteen codes a thread that finds its row itself: 164 us for 120001 rows of 8 heads of 128, bound by its instructions.
+// together). 120001 rows of 8 heads of 128: 132 us, 5.6 TB/s, near the rate of a copy (sixteen codes a thread that finds its row itself: 164 us, bound by
+// its instructions).
 constexpr int kLoadRows = 64;
 template <typename T>
 __global__ void __launch_bounds__(256) load_kernel(const MbFp8Cache c, const int32_t* __restrict__ block_table, int bt_stride,

@@ -394,6 +394,10 @@ def test_store_of_many_tokens(T, n_q, n_kv, d, rot, interleaved):
     (32, 8, 128, 32, [64], [4000]),
     (64, 1, 128, 128, [33, 5], [1900, 3000]),                     # one head for 64
     (12, 4, 128, 128, [65, 1, 129, 7] * 5, [63, 0, 1, 640] * 5),
+    (32, 8, 128, 128, [5] * 16, [125 * i for i in range(16)]),    # short chunks: more than 16 rows of a head, at most 32
+    (6, 1, 64, 16, [5, 3, 1, 4, 5], [900, 3000, 64, 0, 15]),
+    (6, 1, 128, 48, [5, 3, 1, 4, 6], [900, 3000, 64, 0, 15]),     # and one that is not short among them
+    (24, 1, 128, 64, [1] * 5, [63, 64, 2000, 0, 500]),
     (6, 2, 80, 16, [1, 30], [2000, 1500]),                        # a head width of the CUDA cores
 ])
 def test_long_contexts_shared_out(n_q, n_kv, d, page, new, before, dtype):
@@ -421,12 +425,15 @@ def test_values_of_very_different_magnitudes(new, before, d):
 @pytest.mark.parametrize("device", devices())
 @pytest.mark.parametrize("d", [64, 128, 80])
 @pytest.mark.parametrize("n_q,n_kv", [(4, 2), (16, 1), (3, 3)])
-@pytest.mark.parametrize("at", [(1, 40), (0, 3), (2, 69), (2, 68)])
+@pytest.mark.parametrize("at", [(1, 40), (0, 3), (2, 69), (2, 68), (4, 1, 3)])
 def test_nan_reaches_the_rows_that_see_it_and_no_other(at, n_q, n_kv, d, device):
     """A NaN code among the values of one token and head (its column), then among its keys (its row): tokens of the same chunk before it see neither."""
     new, before = [3, 70], [62, 100]
     if device == "cpu":
         new, before = [3, 70], [10, 5]
+    if len(at) == 3:                                  # short chunks
+        new, before = [5 * n_kv, 3 * n_kv, 4 * n_kv], [61, 0, 200]
+        new = [min(n, 32 * n_kv // n_q) for n in new]
     c = case(new, before, n_q, n_kv, d, 16, torch.bfloat16, device, seed=d + n_q)
     key = [before[s] + min(t, new[s] - 1) for s, t in enumerate(at)]
     col, kvh = 13, n_kv - 1
@@ -478,7 +485,7 @@ def test_much_larger_rows_that_come_later(d, dtype, device):
 
 
 @gpu
-@pytest.mark.parametrize("new", [[1] * 4200, [1, 2] * 2100, [210, 213] * 20])
+@pytest.mark.parametrize("new", [[1] * 4200, [1, 2] * 2100, [9, 10] * 1050, [210, 213] * 20])
 def test_more_sequences_and_tiles_than_a_launch_takes(new):
     n_q, n_kv = (64, 1) if len(new) < 100 else (2, 1)
     g = torch.Generator().manual_seed(6)
