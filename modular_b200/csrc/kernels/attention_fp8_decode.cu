@@ -45,6 +45,7 @@ struct Team {
   static constexpr int kWorkers = kPairs * 64;
   static constexpr int kThreads = kWorkers + 32;
   static_assert(kDecStages % kPairs == 0, "stages belong to one pair of warps");
+  static constexpr int kMerge = NR == 1 ? 2 : 4;     // rows of all warps put together at a time
 };
 constexpr int kDecCtas = 2;             // per SM
 constexpr int kMinShare = 2;            // tiles
@@ -319,8 +320,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
   }
   uint8_t* sScale = smem + kDecStages * kStage;     // [stage][K 64 | V 64]
   T* sQ = reinterpret_cast<T*>(sScale + kDecStages * 128);                // [8 NR][HD]: query rows of a piece
-  float* sO = reinterpret_cast<float*>(sQ + 8 * NR * HD);                  // [warp][2 rows][HD + 4]
-  float* sML = sO + kWorkers / 32 * 2 * (HD + 4);                                         // [warp][m 16 | l 16]
+  constexpr int kMerge = Team<NR>::kMerge;
+  float* sO = reinterpret_cast<float*>(sQ + 8 * NR * HD);                  // [warp][kMerge rows][HD + 4]
+  float* sML = sO + kWorkers / 32 * kMerge * (HD + 4);                                         // [warp][m 16 | l 16]
   DecBars& bars = *reinterpret_cast<DecBars*>(sML + kWorkers);
   int* prefix = reinterpret_cast<int*>(&bars + 1);                         // [n_decode + 1]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -537,7 +539,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
       if (++s == kDecStages) { s = 0; ph ^= 1; }
     }
 
-    // ---- the warps' states become one, in the order of the warps, two rows at a time
+    // ---- the warps' states become one, in the order of the warps, kMerge rows at a time
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -551,19 +553,19 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
     float* slot = p.ws + (static_cast<int64_t>(kvh * p.GX + gx) * 2 + (w.ta > 0 ? 0 : 1)) * slot_floats<HD>(p.rows_alloc);
     // (a loop that stays one: fetching straight code that runs once a piece takes longer than running it)
 #pragma unroll 1
-    for (int r0 = 0; r0 < w.rows; r0 += 2) {
-      if (t4 == (r0 & 7) >> 1) {
+    for (int r0 = 0; r0 < w.rows; r0 += kMerge) {
+      if (t4 / (kMerge / 2) == (r0 & 7) / kMerge) {
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const bool up = NR == 2 && r0 >= 8;
-            *reinterpret_cast<float2*>(sO + (warp * 2 + e) * (HD + 4) + c * 16 + 2 * g) =
+            *reinterpret_cast<float2*>(sO + (warp * kMerge + t4 % (kMerge / 2) * 2 + e) * (HD + 4) + c * 16 + 2 * g) =
                 make_float2(up ? st.o[c][NR - 1][e] : st.o[c][0][e], up ? st.o[c][NR - 1][2 + e] : st.o[c][0][2 + e]);
           }
       }
       consumers_sync<kWorkers>();
-      if (tid < HD / 2) {                            // 2 rows of HD / 4 pieces
+      if (tid < kMerge * HD / 4) {                   // rows of HD / 4 pieces
         const int rr = tid / (HD / 4), r = r0 + rr, col = (tid % (HD / 4)) * 4;
         if (r < w.rows) {
           float top = kNoMax, sum = 0.f;
@@ -573,7 +575,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
 #pragma unroll
           for (int q = 0; q < kWorkers / 32; ++q) {
             const float f = exp2f(sML[q * 32 + r] - top);
-            const float4 x = *reinterpret_cast<const float4*>(sO + (q * 2 + rr) * (HD + 4) + col);
+            const float4 x = *reinterpret_cast<const float4*>(sO + (q * kMerge + rr) * (HD + 4) + col);
             sum = fmaf(sML[q * 32 + 16 + r], f, sum);
             v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
           }
@@ -592,8 +594,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
   }
 }
 
-// Sequences that lie in several shares: a block per CTA whose share ends with a sequence's first piece. First every piece's weight, then four groups of 128
-// threads take pieces in turn (one after the other they would cost a round trip to L2 each).
+// Sequences that lie in several shares: blocks per CTA whose share ends with a sequence's first piece, 512 / HD rows each. First every piece's weight, then
+// four groups of 128 threads take pieces in turn (one after the other they would cost a round trip to L2 each).
 template <int HD, typename T>
 __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ DecParams p) {
   constexpr int kPieces = 64;                        // weights kept at a time
@@ -602,7 +604,8 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ DecPa
   pdl_wait();
   const int kvh = blockIdx.y, tid = threadIdx.x, G = p.a.n_q / p.a.n_kv;
   const DecCut cut = p.cuts[kvh * p.GX + blockIdx.x];
-  if (cut.pieces == 0) return;
+  const int q = blockIdx.z * 128 + (threadIdx.x & 127), r = q / (HD / 4), col = (q % (HD / 4)) * 4;      // four columns of a row a thread
+  if (cut.pieces == 0 || blockIdx.z * 128 >= cut.rows * (HD / 4)) return;
   const int qs = cut.qs, rows = cut.rows, n = cut.pieces, group = tid >> 7, lane = tid & 127, half = lane >> 4, r16 = lane & 15;
   // a piece lies in slot 0 of its CTA, the first one, where the sequence begins, in slot 1
   const int64_t slot = slot_floats<HD>(p.rows_alloc);
@@ -624,44 +627,38 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ DecPa
     total[1][tid] = 0.f;
   }
   __syncthreads();
-  for (int q0 = 0; q0 < rows * (HD / 4); q0 += 128) {
-    const int q = q0 + lane, r = q / (HD / 4), col = (q % (HD / 4)) * 4;
-    const bool on = r < rows;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < n; k0 += kPieces) {
-      const int here = min(kPieces, n - k0);
-      if (q0 == 0 || n > kPieces) {
-        __syncthreads();
-        for (int k = tid; k < here * 16; k += 512)
-          if ((k & 15) < rows) {
-            const float* ml = slot_of(k0 + (k >> 4)) + p.rows_alloc * HD + (k & 15);
-            const float f = exp2f(ml[0] - total[0][k & 15]);
-            weight[k >> 4][k & 15] = f;
-            share[k >> 4][k & 15] = f * ml[16];
-          }
-        __syncthreads();
-        if (q0 == 0 && tid < rows)
-          for (int k = 0; k < here; ++k) total[1][tid] += share[k][tid];
+  const bool on = r < rows;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < n; k0 += kPieces) {
+    const int here = min(kPieces, n - k0);
+    __syncthreads();
+    for (int k = tid; k < here * 16; k += 512)
+      if ((k & 15) < rows) {
+        const float* ml = slot_of(k0 + (k >> 4)) + p.rows_alloc * HD + (k & 15);
+        const float f = exp2f(ml[0] - total[0][k & 15]);
+        weight[k >> 4][k & 15] = f;
+        share[k >> 4][k & 15] = f * ml[16];
       }
-      if (on) {
+    __syncthreads();
+    if (tid < rows)
+      for (int k = 0; k < here; ++k) total[1][tid] += share[k][tid];
+    if (on) {
 #pragma unroll 4
-        for (int k = group; k < here; k += 4) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(slot_of(k0 + k) + r * HD + col));
-          const float f = weight[k][r];
-          v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
-        }
+      for (int k = group; k < here; k += 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(slot_of(k0 + k) + r * HD + col));
+        const float f = weight[k][r];
+        v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
       }
     }
-    if (group > 0) sum[group - 1][lane] = v;
-    __syncthreads();
-    const int row = qs + r / G;
-    if (group == 0 && on && row < p.a.T) {
+  }
+  if (group > 0) sum[group - 1][lane] = v;
+  __syncthreads();
+  const int row = qs + r / G;
+  if (group == 0 && on && row < p.a.T) {
 #pragma unroll
-      for (int k = 0; k < 3; ++k) { const float4 x = sum[k][lane]; v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w; }
-      const float l = total[1][r];
-      store4(static_cast<T*>(p.a.out) + static_cast<int64_t>(row) * p.a.ldo + (kvh * G + r % G) * HD + col, v, l == 0.f ? 0.f : 1.f / l);
-    }
-    __syncthreads();
+    for (int k = 0; k < 3; ++k) { const float4 x = sum[k][lane]; v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w; }
+    const float l = total[1][r];
+    store4(static_cast<T*>(p.a.out) + static_cast<int64_t>(row) * p.a.ldo + (kvh * G + r % G) * HD + col, v, l == 0.f ? 0.f : 1.f / l);
   }
 }
 
@@ -676,7 +673,7 @@ template <int HD, int NR, typename T>
 static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cudaStream_t stream) {
   static PerDeviceOnce configured;
   auto kern = decode_kernel<HD, NR, T>;
-  const size_t fixed = kDecStages * (2 * 64 * HD + 128) + 8 * NR * HD * sizeof(T) + (Team<NR>::kWorkers / 32 * 2 * (HD + 4) + Team<NR>::kWorkers) * sizeof(float) + sizeof(DecBars);
+  const size_t fixed = kDecStages * (2 * 64 * HD + 128) + 8 * NR * HD * sizeof(T) + (Team<NR>::kWorkers / 32 * Team<NR>::kMerge * (HD + 4) + Team<NR>::kWorkers) * sizeof(float) + sizeof(DecBars);
   if (configured.needed()) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(fixed + (kMaxDecode + 1) * sizeof(int))) != cudaSuccess)
       return MB_ERR_LAUNCH;
@@ -706,7 +703,7 @@ static int launch(const MbFp8Attention& a, const MbFp8Cache& c, int num_sms, cud
     p.a.n_decode = min(kMaxDecode, a.n_decode - at);
     const size_t smem = fixed + (p.a.n_decode + 1) * sizeof(int);
     if (launch_k(kern, dim3(p.GX, a.n_kv), dim3(Team<NR>::kThreads), smem, stream, tk, tv, p) != cudaSuccess) return MB_ERR_LAUNCH;
-    if (launch_k(join_kernel<HD, T>, dim3(p.GX, a.n_kv), dim3(512), 0, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
+    if (launch_k(join_kernel<HD, T>, dim3(p.GX, a.n_kv, (8 * NR * (HD / 4) + 127) / 128), dim3(512), 0, stream, p) != cudaSuccess) return MB_ERR_LAUNCH;
   }
   return MB_OK;
 }
