@@ -125,7 +125,7 @@ void kv_load_fp8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_s
   }
   check_rc(mb_kv_load_fp8(&c, i32(block_table, 0, k_cache, "block_table"), static_cast<int>(block_table.size(1)), i32(kv_start, B, k_cache, "kv_start"),
                           i32(kv_len, B, k_cache, "kv_len"), static_cast<int>(B), rows, n_kv, hd, k_out.data_ptr(), v_out.data_ptr(),
-                          dtype_code(k_out, "output"), error_flag_on(k_cache.get_device()), cur_stream()),
+                          dtype_code(k_out, "output"), error_flag_on(k_cache.get_device()), num_sms(), cur_stream()),
            "kv_load_fp8");
 }
 

@@ -590,7 +590,7 @@ int mb_rope_kv_store_fp8(const void* qkv, int ld, void* q_out, int ldq, int dtyp
                          const float* cos_sin, int n_positions, const MbFp8Cache* cache, int T, int n_q, int n_kv, int head_dim,
                          int rot_dims, int interleaved, int* err, int num_sms, cudaStream_t stream);
 int mb_kv_load_fp8(const MbFp8Cache* cache, const int32_t* block_table, int bt_stride, const int32_t* kv_start, const int32_t* kv_len,
-                   int B, long long rows, int n_kv, int head_dim, void* k_out, void* v_out, int dtype, int* err, cudaStream_t stream);
+                   int B, long long rows, int n_kv, int head_dim, void* k_out, void* v_out, int dtype, int* err, int num_sms, cudaStream_t stream);
 typedef struct MbFp8Attention {
   const void* q;               // [T, ldq], n_q * head_dim columns first
   void* out;                   // [T, ldo]

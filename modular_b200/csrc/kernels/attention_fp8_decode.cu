@@ -1,7 +1,7 @@
 // Attention of sequences of few rows (single tokens, up to 16 query rows per key/value head) over the 8-bit paged cache.
 //
 // What bounds it is reading the cache: 2 (HD + 1) bytes a token and head, and 24 codes a cycle and SM to unpack on the way. 192 sequences of 2031 tokens
-// on average, 32 over 8 heads of 128: 149 us, 5.4 TB/s (when it took 161, the same loads without the work took 151). Three sequences of 50000: 61 us, 5.1 TB/s. One of 331
+// on average, 32 over 8 heads of 128: 147 us, 5.5 TB/s (when it took 161, the same loads without the work took 151). Three sequences of 50000: 60 us, 5.2 TB/s. One of 331
 // tokens: 10 us, a chain of latencies: lengths, pages, tiles, the join of the pieces in a second launch.
 //
 //   * The 64-token tiles of all sequences are one line of work per head, cut into equal shares (two tiles at least) for as many CTAs
@@ -48,7 +48,7 @@ struct Team {
   static constexpr int kMerge = NR == 1 ? 2 : 4;     // rows of all warps put together at a time
 };
 constexpr int kDecCtas = 2;             // per SM
-constexpr int kMinShare = 2;            // tiles
+constexpr int kMinShare = 2;            // tiles (2 sequences of 3 tokens, 14 rows a head, one tile each: in one share 16.5 us, in two 11.8)
 constexpr int kMaxDecode = 4096;        // sequences of a launch (their tile counts wait in shared memory)
 
 // The sequence whose first piece ends a CTA's share
@@ -124,8 +124,9 @@ __device__ __forceinline__ int tiles_of(const MbFp8Attention& a, int i) {
   if (seq < 0) return 0;
   return (max(a.kv_len[seq], 0) + 63) >> 6;
 }
-// share of CTA g: [U g / G, U (g + 1) / G) with G the CTAs that get at least kMinShare tiles
-__device__ __forceinline__ int shares_of(int U, int GX) { return max(1, min(GX, U / kMinShare)); }
+// share of CTA g: [U g / G, U (g + 1) / G) with G the CTAs that get at least kMinShare tiles, or one for each of n sequences: pairs of warps work on the tiles
+// of a sequence side by side, on sequences one after the other
+__device__ __forceinline__ int shares_of(int U, int GX, int n) { return max(1, min(GX, max(U / kMinShare, min(n, U)))); }
 __device__ __forceinline__ int share_start(int U, int G, int g) { return static_cast<int>(static_cast<int64_t>(U) * g / G); }
 __device__ __forceinline__ int share_holding(int U, int G, int u) { return static_cast<int>(((static_cast<int64_t>(u) + 1) * G - 1) / U); }
 
@@ -359,7 +360,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
   }
   if (tid == 0) prefix[nd] = run;
   __syncthreads();
-  const int U = run, GE = shares_of(U, p.GX), gx = blockIdx.x;
+  const int U = run, GE = shares_of(U, p.GX, nd), gx = blockIdx.x;
   if (bare && gx == 0) {
     // their rows are zero
     for (int i = 0; i < nd; ++i) {
@@ -391,7 +392,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
   volatile int* abort_word = &bars.abort_word;
 
   if (warp == kWorkers / 32) {
-    // ---------------------------------------------------------------- producer: 32 lanes fetch page numbers, lane 0 issues
+    // ---------------------------------------------------------------- producer: 32 lanes fetch page numbers, up to 16 issue
     const int per = 64 / p.box;                     // boxes of a tile
     int s = 0, n = 0;
     uint32_t ph = 0;
@@ -422,35 +423,38 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
                     &bars.q_full);
         ++n;
       }
-      int page_lane = 0, have = 0, at = 0;          // pages of the next 32 boxes
-      for (int t = u - fu; t < t1; ++t) {
-        const int left = kl - t * 64, boxes = min(per, (left + p.box - 1) / p.box);
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], ph ^ 1, abort_word, p.a.err, 741));
-        if (!ok) break;
-        uint8_t* dst = smem + s * kStage;
-        if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], static_cast<uint32_t>(boxes) * p.box * (2 * HD + 2));
-        for (int c = 0; c < boxes; ++c, ++at) {
-          if (at == have) {
-            at = 0;
-            have = 32;
-            const int tok = t * 64 + (c + lane) * p.box, nth = tok / p.c.page_size;
-            page_lane = 0;
-            if (tok < kl) {
-              page_lane = nth < p.a.bt_stride ? bt[nth] : -1;
-              if (page_lane < 0 || page_lane >= p.c.pages) {       // reported; some page stands in for it
-                if (p.a.err) atomicCAS(p.a.err, 0, 731);
-                page_lane = 0;
-              }
+      int page_lane = 0, off_lane = 0, at = 32;     // places of the next 32 boxes
+      for (int t = u - fu; t < t1; ++t, at += per) {
+        if (at == 32) {
+          at = 0;
+          const int tok = t * 64 + lane * p.box, nth = tok / p.c.page_size;
+          off_lane = tok - nth * p.c.page_size;
+          page_lane = 0;
+          if (tok < kl) {
+            page_lane = nth < p.a.bt_stride ? bt[nth] : -1;
+            if (page_lane < 0 || page_lane >= p.c.pages) {         // reported; some page stands in for it
+              if (p.a.err) atomicCAS(p.a.err, 0, 731);
+              page_lane = 0;
             }
           }
-          const int page = __shfl_sync(0xffffffffu, page_lane, at);
-          if (lane == 0) {
-            const int off = (t * 64 + c * p.box) % p.c.page_size;
-            tma_load_4d(dst + c * p.box * HD, &tmK, &bars.full[s], 0, off, kvh, page);
-            tma_load_4d(dst + kCodes + c * p.box * HD, &tmV, &bars.full[s], 0, off, kvh, page);
-            bulk_load(sScale + s * 128 + c * p.box, p.c.ks + page * p.c.ks_page + kvh * p.c.ks_head + off, p.box, &bars.full[s]);
-            bulk_load(sScale + s * 128 + 64 + c * p.box, p.c.vs + page * p.c.vs_page + kvh * p.c.vs_head + off, p.box, &bars.full[s]);
-          }
+        }
+        const int left = kl - t * 64, boxes = min(per, (left + p.box - 1) / p.box), c = per == 1 ? 0 : lane >> 2;
+        const int page = __shfl_sync(0xffffffffu, page_lane, min(at + c, 31)), off = __shfl_sync(0xffffffffu, off_lane, min(at + c, 31));
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], ph ^ 1, abort_word, p.a.err, 741));
+        if (!ok) break;
+        uint8_t* dst = smem + s * kStage + c * p.box * HD;
+        uint8_t* dst_e = sScale + s * 128 + c * p.box;
+        if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], static_cast<uint32_t>(boxes) * p.box * (2 * HD + 2));
+        // One lane issues a tile's four copies; where a page ends inside a tile there are more, a lane each (pages of 48 tokens, 8 sequences of 15 tokens over 40
+        // heads of their own, 8278 tokens: 47 -> 36 us; with whole tiles a lane each is 1 % slower)
+        const bool one = per == 1;
+        if (!one) __syncwarp();
+        if (one ? lane == 0 : c < boxes) {
+          const int kind = one ? -1 : lane & 3;
+          if (one || kind == 0) tma_load_4d(dst, &tmK, &bars.full[s], 0, off, kvh, page);
+          if (one || kind == 1) tma_load_4d(dst + kCodes, &tmV, &bars.full[s], 0, off, kvh, page);
+          if (one || kind == 2) bulk_load(dst_e, p.c.ks + page * p.c.ks_page + kvh * p.c.ks_head + off, p.box, &bars.full[s]);
+          if (one || kind == 3) bulk_load(dst_e + 64, p.c.vs + page * p.c.vs_page + kvh * p.c.vs_head + off, p.box, &bars.full[s]);
         }
         if (++s == kDecStages) { s = 0; ph ^= 1; }
       }

@@ -343,15 +343,15 @@ static int launch_store(const StoreParams& p, int num_sms, cudaStream_t stream) 
   return launch_k(kern, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p) == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;
 }
 
-// Rows [0, kv_len[s]) of every sequence at kv_start[s] of the outputs; rows that belong to no sequence are zeros. A block takes 64 rows of all heads,
-// keys or values by grid.y: it looks each row's place up once, then eight codes a thread, a head at a time (the tokens of a page and head lie
+// Rows [0, kv_len[s]) of every sequence at kv_start[s] of the outputs; rows that belong to no sequence are zeros. A block takes 64 rows,
+// keys or values by grid.y, of all heads, or of some by grid.z where there are few rows: it looks each row's place up once, then eight codes a thread, a head at a time (the tokens of a page and head lie
 // together). 120001 rows of 8 heads of 128: 132 us, 5.6 TB/s, near the rate of a copy (sixteen codes a thread that finds its row itself: 164 us, bound by
 // its instructions).
 constexpr int kLoadRows = 64;
 template <typename T>
 __global__ void __launch_bounds__(256) load_kernel(const MbFp8Cache c, const int32_t* __restrict__ block_table, int bt_stride,
                                                    const int32_t* __restrict__ kv_start, const int32_t* __restrict__ kv_len, int B, int64_t rows,
-                                                   int n_kv, int hd, T* __restrict__ k_out, T* __restrict__ v_out, int* err) {
+                                                   int n_kv, int hd, int heads, T* __restrict__ k_out, T* __restrict__ v_out, int* err) {
   __shared__ int64_t s_codes[kLoadRows], s_byte[kLoadRows];                  // < 0: a row of nobody
   pdl_wait();
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kLoadRows;
@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(256) load_kernel(const MbFp8Cache c, const int
   const int64_t c_head = is_v ? c.v_head : c.k_head, b_head = is_v ? c.vs_head : c.ks_head;
   T* out = (is_v ? v_out : k_out) + row0 * n_kv * hd + col;
   const int n = static_cast<int>(rows - row0 < kLoadRows ? rows - row0 : kLoadRows);
-  for (int h = 0; h < n_kv; ++h) {
+  const int h0 = blockIdx.z * heads, h1 = min(h0 + heads, n_kv);
+  for (int h = h0; h < h1; ++h) {
     for (int r0 = sub; r0 < n; r0 += 4 * step) {
       uint2 w[4];
       uint8_t e[4];
@@ -456,7 +457,8 @@ extern "C" int mb_rope_kv_store_fp8(const void* qkv, int ld, void* q_out, int ld
 }
 
 extern "C" int mb_kv_load_fp8(const MbFp8Cache* cache, const int32_t* block_table, int bt_stride, const int32_t* kv_start, const int32_t* kv_len,
-                              int B, long long rows, int n_kv, int head_dim, void* k_out, void* v_out, int dtype, int* err, cudaStream_t stream) {
+                              int B, long long rows, int n_kv, int head_dim, void* k_out, void* v_out, int dtype, int* err, int num_sms,
+                              cudaStream_t stream) {
   using namespace mb::kv8;
   if (rows <= 0) return MB_OK;
   const int rc = check_cache(cache, n_kv, head_dim);
@@ -464,12 +466,15 @@ extern "C" int mb_kv_load_fp8(const MbFp8Cache* cache, const int32_t* block_tabl
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return MB_ERR_ALIGN;
   const long long blocks = (rows + kLoadRows - 1) / kLoadRows;
   if (blocks > 0x7fffffff) return MB_ERR_TOO_LARGE;
-  const dim3 grid(static_cast<unsigned>(blocks), 2);
+  // heads of a block: all where that makes four blocks an SM, else as few as it takes (30 rows of 40 heads in two blocks: 26 us, in 80 2.8)
+  int heads = n_kv;
+  while (heads > 1 && 2 * blocks * ((n_kv + heads - 1) / heads) < 4ll * num_sms) heads = (heads + 1) / 2;
+  const dim3 grid(static_cast<unsigned>(blocks), 2, static_cast<unsigned>((n_kv + heads - 1) / heads));
   cudaError_t e;
   switch (dtype) {
-    case 0: e = launch_k(load_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, *cache, block_table, bt_stride, kv_start, kv_len, B, rows, n_kv, head_dim, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), err); break;
-    case 1: e = launch_k(load_kernel<float>, grid, dim3(256), 0, stream, *cache, block_table, bt_stride, kv_start, kv_len, B, rows, n_kv, head_dim, static_cast<float*>(k_out), static_cast<float*>(v_out), err); break;
-    case 2: e = launch_k(load_kernel<__half>, grid, dim3(256), 0, stream, *cache, block_table, bt_stride, kv_start, kv_len, B, rows, n_kv, head_dim, static_cast<__half*>(k_out), static_cast<__half*>(v_out), err); break;
+    case 0: e = launch_k(load_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, *cache, block_table, bt_stride, kv_start, kv_len, B, rows, n_kv, head_dim, heads, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), err); break;
+    case 1: e = launch_k(load_kernel<float>, grid, dim3(256), 0, stream, *cache, block_table, bt_stride, kv_start, kv_len, B, rows, n_kv, head_dim, heads, static_cast<float*>(k_out), static_cast<float*>(v_out), err); break;
+    case 2: e = launch_k(load_kernel<__half>, grid, dim3(256), 0, stream, *cache, block_table, bt_stride, kv_start, kv_len, B, rows, n_kv, head_dim, heads, static_cast<__half*>(k_out), static_cast<__half*>(v_out), err); break;
     default: return MB_ERR_SHAPE;
   }
   return e == cudaSuccess ? MB_OK : MB_ERR_LAUNCH;

@@ -443,7 +443,8 @@ def rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale,
     else:
         _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, n_kv, head_dim)
         ref.rope_kv_store_fp8(qkv, positions, slots, cos_sin, k_cache, v_cache, k_scale, v_scale, n_q, n_kv, head_dim, interleaved, rot, q)
-    return q[: qkv.shape[0], : n_q * head_dim]
+    shape = (qkv.shape[0], n_q * head_dim)
+    return q if q.shape == shape else q[: shape[0], : shape[1]]
 
 
 def kv_load_fp8(k_cache, v_cache, k_scale, v_scale, block_table, kv_start, kv_len, rows, dtype=torch.bfloat16, out=None):
