@@ -40,9 +40,15 @@ def gemm_workspace(device) -> torch.Tensor:
     return ws
 
 
+_DEVICE_CHECKS = {721: "a position out of range", 722: "a slot out of range", 723: "a page out of range in a load", 731: "a page out of range in attention",
+                  732: "an attention plan of other sequences"}
+
+
 def check_device_error() -> None:
-    """Raises if a kernel reported a timed-out wait (reads and clears the error word)."""
+    """Raises if a kernel reported a timed-out wait or an index out of range (reads and clears the error word)."""
     code = _lib().read_error_flag(True)
+    if code in _DEVICE_CHECKS:
+        raise RuntimeError(f"modular_b200 kernel reported {_DEVICE_CHECKS[code]} (code {code})")
     if code:
         raise RuntimeError(f"modular_b200 kernel reported a bounded-wait timeout (code {code})")
 

@@ -705,16 +705,16 @@ def test_pages_slots_and_positions_out_of_range_are_reported():
     k, v, ks, vs = cache.views
     cache.kv.fill_(0x38)
     one = lambda *a: ints(a, "cuda")  # noqa: E731
-    for pos, slot in (([0, 9, 1], [0, 1, 2]), ([0, -1, 1], [0, 1, 2]), ([0, 1, 2], [0, 64, 2])):
+    for pos, slot, what in (([0, 9, 1], [0, 1, 2], "position"), ([0, -1, 1], [0, 1, 2], "position"), ([0, 1, 2], [0, 64, 2], "slot")):
         ops.rope_kv_store_fp8(qkv, one(*pos), torch.tensor(slot, device="cuda"), cs, k, v, ks, vs, 4, 2, 64)
         torch.cuda.synchronize()
-        with pytest.raises(RuntimeError):
+        with pytest.raises(RuntimeError, match=what):
             ops.check_device_error()
     for table in ([[99]], [[-3]]):
         for n in (1, 3):
             ops.paged_attention_fp8(qkv[:n].contiguous(), k, v, ks, vs, ints(table, "cuda"), one(0), one(n), one(5), 4, 2, 64, 0.1)
             torch.cuda.synchronize()
-            with pytest.raises(RuntimeError):
+            with pytest.raises(RuntimeError, match="page"):
                 ops.check_device_error()
     ops.paged_attention_fp8(qkv, k, v, ks, vs, ints([[0]], "cuda"), one(0), one(3), one(40), 4, 2, 64, 0.1)      # more keys than pages
     torch.cuda.synchronize()
