@@ -599,70 +599,65 @@ decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ C
 }
 
 // Sequences that lie in several shares: blocks per CTA whose share ends with a sequence's first piece, 512 / HD rows each. First every piece's weight, then
-// four groups of 128 threads take pieces in turn (one after the other they would cost a round trip to L2 each).
+// four groups of 128 threads take pieces in turn (one after the other they would cost a round trip to L2 each), their first already on its way.
 template <int HD, typename T>
 __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ DecParams p) {
-  constexpr int kPieces = 64;                        // weights kept at a time
-  __shared__ float weight[kPieces][16], share[kPieces][16], total[2][16];     // of a piece's values, and times its sum
+  constexpr int kPieces = 32;                        // weights kept at a time
+  __shared__ float largest[kPieces][16], weight[kPieces][16], share[kPieces][16];      // share: of the sum
   __shared__ float4 sum[3][128];
   pdl_wait();
   const int kvh = blockIdx.y, tid = threadIdx.x, G = p.a.n_q / p.a.n_kv;
   const DecCut cut = p.cuts[kvh * p.GX + blockIdx.x];
-  const int q = blockIdx.z * 128 + (threadIdx.x & 127), r = q / (HD / 4), col = (q % (HD / 4)) * 4;      // four columns of a row a thread
+  const int q = blockIdx.z * 128 + (tid & 127), r = q / (HD / 4), col = (q % (HD / 4)) * 4;      // four columns of a row a thread
   if (cut.pieces == 0 || blockIdx.z * 128 >= cut.rows * (HD / 4)) return;
-  const int qs = cut.qs, rows = cut.rows, n = cut.pieces, group = tid >> 7, lane = tid & 127, half = lane >> 4, r16 = lane & 15;
+  const int rows = cut.rows, n = cut.pieces, group = tid >> 7, lane = tid & 127;
+  const bool on = r < rows;
   // a piece lies in slot 0 of its CTA, the first one, where the sequence begins, in slot 1
   const int64_t slot = slot_floats<HD>(p.rows_alloc);
   const float* base = p.ws + (static_cast<int64_t>(kvh) * p.GX + blockIdx.x) * 2 * slot;
   auto slot_of = [&](int k) { return base + (2 * k + (k == 0 ? 1 : 0)) * slot; };
-  // the largest reference of each row
-  if (group == 0) {
-    float m = kNoMax;
-    if (r16 < rows)
-      for (int k = half; k < n; k += 8) m = fmaxf(m, slot_of(k)[p.rows_alloc * HD + r16]);
-    sum[0][lane].x = m;
-  }
+  auto values = [&](int k) { return __ldcg(reinterpret_cast<const float4*>(slot_of(k) + r * HD + col)); };
+  // a thread per piece and row: reference and sum. The group's first values are on their way with them.
+  const int piece = tid >> 4, r16 = tid & 15;
+  auto reference = [&](int k) { return k < n && r16 < rows ? slot_of(k)[p.rows_alloc * HD + r16] : kNoMax; };
+  auto part = [&](int k) { return k < n && r16 < rows ? slot_of(k)[p.rows_alloc * HD + 16 + r16] : 0.f; };
+  float m = reference(piece), l = part(piece);
+  const float4 first = on && group < n ? values(group) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float top = m;
+  for (int k = piece + kPieces; k < n; k += kPieces) top = fmaxf(top, reference(k));
+  largest[piece][r16] = top;
   __syncthreads();
-  if (tid < 16) {
-    float m = kNoMax;
-#pragma unroll
-    for (int h = 0; h < 8; ++h) m = fmaxf(m, sum[0][h * 16 + tid].x);
-    total[0][tid] = m;
-    total[1][tid] = 0.f;
-  }
-  __syncthreads();
-  const bool on = r < rows;
+  for (int k = 0; k < min(n, kPieces); ++k) top = fmaxf(top, largest[k][r16]);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
   for (int k0 = 0; k0 < n; k0 += kPieces) {
     const int here = min(kPieces, n - k0);
-    __syncthreads();
-    for (int k = tid; k < here * 16; k += 512)
-      if ((k & 15) < rows) {
-        const float* ml = slot_of(k0 + (k >> 4)) + p.rows_alloc * HD + (k & 15);
-        const float f = exp2f(ml[0] - total[0][k & 15]);
-        weight[k >> 4][k & 15] = f;
-        share[k >> 4][k & 15] = f * ml[16];
-      }
-    __syncthreads();
-    if (tid < rows)
-      for (int k = 0; k < here; ++k) total[1][tid] += share[k][tid];
-    if (on) {
-#pragma unroll 4
-      for (int k = group; k < here; k += 4) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(slot_of(k0 + k) + r * HD + col));
-        const float f = weight[k][r];
-        v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
-      }
+    if (k0 > 0) {
+      __syncthreads();
+      m = reference(k0 + piece);
+      l = part(k0 + piece);
     }
+    const float f = exp2f(m - top);
+    weight[piece][r16] = f;
+    share[piece][r16] = f * l;
+    __syncthreads();
+    if (!on) continue;
+#pragma unroll 4
+    for (int k = group; k < here; k += 4) {
+      const float4 x = k0 == 0 && k == group ? first : values(k0 + k);
+      const float w = weight[k][r];
+      v.x = fmaf(x.x, w, v.x); v.y = fmaf(x.y, w, v.y); v.z = fmaf(x.z, w, v.z); v.w = fmaf(x.w, w, v.w);
+    }
+    if (group == 0)
+      for (int k = 0; k < here; ++k) total += share[k][r];
   }
   if (group > 0) sum[group - 1][lane] = v;
   __syncthreads();
-  const int row = qs + r / G;
+  const int row = cut.qs + r / G;
   if (group == 0 && on && row < p.a.T) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) { const float4 x = sum[k][lane]; v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w; }
-    const float l = total[1][r];
-    store4(static_cast<T*>(p.a.out) + static_cast<int64_t>(row) * p.a.ldo + (kvh * G + r % G) * HD + col, v, l == 0.f ? 0.f : 1.f / l);
+    store4(static_cast<T*>(p.a.out) + static_cast<int64_t>(row) * p.a.ldo + (kvh * G + r % G) * HD + col, v, total == 0.f ? 0.f : 1.f / total);
   }
 }
 
