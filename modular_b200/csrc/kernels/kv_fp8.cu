@@ -74,11 +74,12 @@ __device__ __forceinline__ float turned(float a, float c, float b, float s) {
   const float p = a * c, q = b * s;
   const float sum = p + q, back = sum - p;
   const float rest = ((p - (sum - back)) + (q - back)) + (fmaf(a, c, -p) + fmaf(b, s, -q));
-  const float r = sum + rest;
-  if (!(fabsf(r) <= 3.0e38f)) return sum;           // not finite
-  const float d = (sum - r) + rest;
+  const float r = sum + rest;                       // (where the sum is infinite this is NaN, which is what it is held as)
   uint32_t u = __float_as_uint(r);
-  if (d != 0.f && (u & 0x7fffu) == 0 && r != 0.f) u += ((d > 0.f) == (r > 0.f)) ? 1u : 0xffffffffu;
+  if (__builtin_expect((u & 0x7fffu) == 0, 0)) {
+    const float d = (sum - r) + rest;
+    if (d != 0.f && r != 0.f) u += ((d > 0.f) == (r > 0.f)) ? 1u : 0xffffffffu;
+  }
   return __uint_as_float(u);
 }
 
@@ -108,11 +109,18 @@ __device__ __forceinline__ int row_exponent(float big) {
   const uint32_t u = __float_as_uint(big);
   return max(static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0), kLeastExp);
 }
-__device__ __forceinline__ float largest(const float (&x)[8], float big) {
+// The largest finite magnitude; infinities become NaN. (A maximum leaves NaN out, so that one comparison for all finds them.)
+__device__ __forceinline__ float largest(float (&x)[8]) {
+  float big = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(x[i]);
-    big = fmaxf(big, a < INFINITY ? a : 0.f);       // (NaN compares false)
+  for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[i]));
+  if (__builtin_expect(big == INFINITY, 0)) {
+    big = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (fabsf(x[i]) == INFINITY) x[i] = NAN;
+      big = fmaxf(big, fabsf(x[i]));
+    }
   }
   return big;
 }
@@ -120,9 +128,7 @@ __device__ __forceinline__ uint2 quantised(const float (&x)[8], float inv) {
   uint32_t w[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    float2 f;
-    f.x = fabsf(x[2 * k]) < INFINITY ? x[2 * k] * inv : NAN;
-    f.y = fabsf(x[2 * k + 1]) < INFINITY ? x[2 * k + 1] * inv : NAN;
+    const float2 f = make_float2(x[2 * k] * inv, x[2 * k + 1] * inv);
     w[k] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
   }
   return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
@@ -190,7 +196,7 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreParams p) {
   if (h < p.n_q) {
     if (on) store8(static_cast<T*>(p.q_out) + static_cast<int64_t>(t) * p.ldq + static_cast<int64_t>(h) * p.hd + col, x);
   }
-  float big = largest(x, 0.f);
+  float big = largest(x);
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
   if (!on || h < p.n_q) return;
@@ -210,10 +216,10 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreParams p) {
 
 // Heads of 64, 128 or 256 whose pairs lie in whole groups of eight. HD / 16 lanes hold a row, each two groups of eight columns: the two halves of eight
 // pairs, or two neighbouring groups. A warp takes one token and walks over some of its rows, 32 / LANES at a time, with the angles in registers: they
-// are read once for all heads. The next rows are on their way while a step's are worked on. 8192 tokens of 32 + 2 x 8 heads of 128: 45 us, 4.2 TB/s (a
-// thread an element group with its own angles: 108 us; rows fetched when they are needed: 65). What bounds it is not the memory but how much of it eight
-// warps an SM quarter keep on the way beside the exact rotation of keys; more blocks with fewer registers were slower. 64 tokens: 5 us, the latency of
-// position, angles and row one after the other.
+// are read once for all heads. The next rows are on their way while a step's are worked on. 8192 tokens of 32 + 2 x 8 heads of 128: 39.5 us, 4.8 TB/s (a
+// thread an element group with its own angles: 108 us; rows fetched when they are needed: 65; what is rare, infinities and short sums, looked at for each value
+// and not in branches: 45). What bounds it is the instructions of keys and values beside loads that six warps an SM quarter keep on their way; more blocks with
+// fewer registers were slower. 64 tokens: 3.8 us, the latency of position, angles and row one after the other.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) store_rows_kernel(const StoreParams p, int per_warp) {
   constexpr int LANES = HD / 16, RPW = 32 / LANES;
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) store_rows_kernel
         }
       }
       if (hb - sub + u * RPW + RPW <= p.n_q) continue;                        // (of the whole warp) queries only
-      float big = largest(b, largest(a, 0.f));
+      float big = fmaxf(largest(a), largest(b));
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
       if (h >= h1 || h < p.n_q || slot < 0) continue;
